@@ -51,6 +51,14 @@ typedef enum yh_status {
     YH_ERR_ALIGN = -6
 } yh_status;
 
+/* Element types of the row operators below (the head path is float32 throughout). */
+typedef enum yh_dtype {
+    YH_FLOAT32 = 0,
+    YH_BFLOAT16 = 1,
+    YH_FLOAT16 = 2,
+    YH_INT8 = 3
+} yh_dtype;
+
 /* bits of the per-image device-side status words written by yh_detect / yh_nms */
 #define YH_STATUS_CANDIDATE_OVERFLOW 1 /* an image had more candidates than max_candidates; result invalid for it */
 #define YH_STATUS_COUNT_SHIFT 8        /* with the overflow bit: bits 8..30 = the image's candidates / 256, rounded up
@@ -364,6 +372,103 @@ int yh_loss_with_grad(const yh_head_config *cfg, const float *const *heads, cons
                       int32_t normalize_by_num_gt, void *workspace, size_t workspace_bytes,
                       float *loss_per_image, float *loss_parts, float *iou_max, float *loss_sum,
                       const float *grad_per_image, float *const *grad_heads, void *stream);
+
+/* ---- row operators in 8 bits ------------------------------------------------
+ * For the convolution stack around the head path: a "row" is one pixel of an NHWC
+ * activation, its K (or C) channels.  No counterpart in the reference, whose
+ * convolutions and batch normalisation are TensorFlow's.
+ *
+ * Common rules
+ *  - matrices are rows x channels, channels adjacent, `ld*` elements from one row
+ *    to the next: at least the number of channels for outputs, not negative for
+ *    inputs (0: one row for all).  A pointer is aligned to its element, nothing
+ *    more is asked; multiples of 16 bytes are faster.  What lies between the rows
+ *    or behind the last one is neither read nor written.
+ *  - x, y, dy, dx, z, a, da, dz are YH_FLOAT32, YH_BFLOAT16 or YH_FLOAT16 (one type
+ *    a call unless said otherwise); scales, vectors per channel, dw and db are
+ *    float32.  Results of 16 bits are rounded once from float32.
+ *  - outputs do not overlap inputs unless said otherwise; workspaces are plain
+ *    scratch (nothing is expected in them and nothing kept), 16-byte aligned, and
+ *    may be NULL where the size query says 0; calls that overlap in time need
+ *    workspaces of their own.  No call allocates, clears with a memset or uses
+ *    atomics: every call can be captured into a graph, and gives the same bits on
+ *    every run.
+ *  - 0 <= rows < YH_MAX_ROWS, 1 <= channels <= YH_MAX_ROW_CHANNELS, and the product
+ *    of any two of a call's sizes is below 2^38 (weights: below 2^31).
+ *
+ * Codes of a row: scale = max|x| / 127 in float32, code = x * r rounded half to even
+ * from the exact product, r = 127 / max|x| in float32; the value a code stands for
+ * is code * scale.  A row whose largest magnitude is below 2^-110 is zero (scale 0).
+ * A row that holds an infinity or a NaN has the scale NaN and codes 0: all that is
+ * computed from it is NaN. */
+#define YH_MAX_ROWS (1 << 26)
+#define YH_MAX_ROW_CHANNELS (1 << 16)
+
+/* codes [rows][k] int8, scale [rows], of x [rows][k]. */
+int yh_quantize_rows(const void *x, int32_t dtype, int64_t ldx, int64_t rows, int32_t k,
+                     int8_t *codes, int64_t ldc, float *scale, void *stream);
+/* x [rows][k] = codes * scale. */
+int yh_dequantize_rows(const int8_t *codes, int64_t ldc, const float *scale, int64_t rows, int32_t k,
+                       void *x, int32_t dtype, int64_t ldx, void *stream);
+
+/* A pointwise (1x1) convolution in 8-bit integers:
+ *   y[m][c] = (sum_k code(x)[m][k] * w[c][k]) * scale(x)[m] * w_scale[c] + bias[c]
+ * with an exact sum in 32 bits.
+ *   x         [rows][k] of x_dtype: its codes are taken within the call; or
+ *             YH_INT8 codes, whose scales come in x_scale [rows] (else NULL);
+ *   w [n][k]  int8 codes of the weights' rows (yh_quantize_rows), w_scale [n];
+ *   bias [n]  may be NULL;
+ *   codes [rows][k], scale [rows]: where the codes of x are left for the backward
+ *             pass; both NULL if they are not wanted, or if x is YH_INT8. */
+int yh_matmul_int8_workspace_bytes(int64_t rows, int32_t k, int32_t n, int32_t x_dtype, int32_t want_codes, size_t *bytes);
+int yh_matmul_int8(const void *x, int32_t x_dtype, int64_t ldx, const float *x_scale, int64_t rows, int32_t k,
+                   const int8_t *w, int64_t ldw, const float *w_scale, int32_t n, const float *bias,
+                   void *y, int32_t y_dtype, int64_t ldy, int8_t *codes, int64_t ldc, float *scale,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* Gradient of that product (or of any product whose input is kept as codes) with
+ * respect to the weights and the bias:
+ *   dw[c][k] = sum_m dy[m][c] * scale[m] * codes[m][k],  db[c] = sum_m dy[m][c]
+ * dw [n][k] float32, adjacent rows; db [n] may be NULL.  The terms are exact to
+ * float32 and the sums float32 within a piece of the rows, 64 bits over the pieces.
+ * An infinity in dy counts as a NaN.  rows = 0 gives zeros. */
+int yh_weight_grad_workspace_bytes(int64_t rows, int32_t n, int32_t k, size_t *bytes);
+int yh_weight_grad(const void *dy, int32_t dtype, int64_t lddy, const int8_t *codes, int64_t ldc, const float *scale,
+                   int64_t rows, int32_t n, int32_t k, float *dw, float *db,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* Gradient with respect to the input, rounding taken as the identity:
+ *   dx[m][k] = sum_c dy[m][c] * w_scale[c] * w[c][k]
+ * dx [rows][k] has dy's type.  An infinity in dy counts as a NaN. */
+int yh_input_grad(const void *dy, int32_t dtype, int64_t lddy, const int8_t *w, int64_t ldw, const float *w_scale,
+                  int64_t rows, int32_t n, int32_t k, void *dx, int64_t lddx, void *stream);
+
+/* Batch normalisation on the batch's own statistics, leaky ReLU and a shortcut:
+ *   mean[c], var[c] over the rows of z (in 64 bits), invstd = 1 / sqrt(var + eps),
+ *   xhat = (z - mean) * invstd,  u = xhat * gamma + beta,
+ *   a = (u > 0 ? u : slope * u) + residual            (slope 1: no activation)
+ * and its checkpoint, one byte an element: the side of u in the lowest bit, exactly,
+ * and above it xhat in seven bits, relative to the row's largest |xhat| (scale = that
+ * / 63).  The backward pass reads the checkpoint in the place of z, u and a:
+ *   du = u > 0 ? da : slope * da,  dbeta = sum du,  dgamma = sum du * xq,
+ *   dz = gamma * invstd * (du - dbeta / rows - xq * dgamma / rows),
+ * xq being the value that the checkpoint holds; the residual's gradient is da.
+ *   residual, kept with scale, running_mean with running_var: may be NULL;
+ *   running_* [c]: (1 - momentum) * running + momentum * (mean, var * rows / (rows - 1));
+ *   mean, invstd [c]: outputs, invstd is read by the backward pass;
+ *   rows >= 1 (one row: var is 0).  The statistics of a channel that holds an
+ *   infinity or a NaN are NaN, and with them everything but the other channels' a.
+ * a may be residual, dz may be da (the same rows in place). */
+int yh_norm_act_workspace_bytes(int64_t rows, int32_t c, int32_t dtype, size_t *bytes);
+int yh_norm_act_forward(const void *z, int64_t ldz, const void *residual, int64_t ldr, int32_t dtype, int64_t rows, int32_t c,
+                        const float *gamma, const float *beta, double eps, float slope,
+                        void *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale, float *mean, float *invstd,
+                        float *running_mean, float *running_var, double momentum,
+                        void *workspace, size_t workspace_bytes, void *stream);
+int yh_norm_act_backward(const void *da, int64_t ldda, int32_t dtype, int64_t rows, int32_t c,
+                         const int8_t *kept, int64_t ldk, const float *scale, const float *gamma, const float *invstd, float slope,
+                         void *dz, int64_t lddz, float *dgamma, float *dbeta,
+                         void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,10 @@ YH_STATUS_CANDIDATE_OVERFLOW = 1
 YH_STATUS_COUNT_SHIFT = 8
 YH_STATIC_SCRATCH_BYTES = 8 << 20
 
+YH_MAX_ROWS = 1 << 26
+YH_MAX_ROW_CHANNELS = 1 << 16
+YH_FLOAT32, YH_BFLOAT16, YH_FLOAT16, YH_INT8 = 0, 1, 2, 3
+
 YH_OK = 0
 YH_ERR_INVALID_ARG = -1
 YH_ERR_NO_DEVICE = -2
@@ -53,7 +57,11 @@ class Tuning(ctypes.Structure):
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
+_L = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
+_N = ctypes.c_size_t
+_PN = ctypes.POINTER(ctypes.c_size_t)
 _CFG = ctypes.POINTER(HeadConfig)
 _PP = ctypes.POINTER(ctypes.c_void_p)
 
@@ -92,6 +100,17 @@ SIGNATURES = {
                                          _P, _P, _P, _P, _P, _PP, _P]),
     'yh_loss': (ctypes.c_int, [_CFG, _PP, _P, _I, _I, ctypes.POINTER(_F), _F, _I, _P, ctypes.c_size_t,
                                _P, _P, _P, _P, _P]),
+    'yh_quantize_rows': (ctypes.c_int, [_P, _I, _L, _L, _I, _P, _L, _P, _P]),
+    'yh_dequantize_rows': (ctypes.c_int, [_P, _L, _P, _L, _I, _P, _I, _L, _P]),
+    'yh_matmul_int8_workspace_bytes': (ctypes.c_int, [_L, _I, _I, _I, _I, _PN]),
+    'yh_matmul_int8': (ctypes.c_int, [_P, _I, _L, _P, _L, _I, _P, _L, _P, _I, _P, _P, _I, _L, _P, _L, _P, _P, _N, _P]),
+    'yh_weight_grad_workspace_bytes': (ctypes.c_int, [_L, _I, _I, _PN]),
+    'yh_weight_grad': (ctypes.c_int, [_P, _I, _L, _P, _L, _P, _L, _I, _I, _P, _P, _P, _N, _P]),
+    'yh_input_grad': (ctypes.c_int, [_P, _I, _L, _P, _L, _P, _L, _I, _I, _P, _L, _P]),
+    'yh_norm_act_workspace_bytes': (ctypes.c_int, [_L, _I, _I, _PN]),
+    'yh_norm_act_forward': (ctypes.c_int, [_P, _L, _P, _L, _I, _L, _I, _P, _P, _D, _F, _P, _L, _P, _L, _P, _P, _P,
+                                           _P, _P, _D, _P, _N, _P]),
+    'yh_norm_act_backward': (ctypes.c_int, [_P, _L, _I, _L, _I, _P, _L, _P, _P, _P, _F, _P, _L, _P, _P, _P, _N, _P]),
 }
 
 _lib = None

@@ -11,6 +11,7 @@
 #include <limits>
 #include <mutex>
 #include "yh_internal.h"
+#include "yh_rows.h"
 
 namespace {
 
@@ -447,6 +448,20 @@ int compute_units()
 }
 
 }  // namespace
+
+// For the entry points of other files (yh_rows.h).
+namespace yh {
+int report(int code, const char *fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+int report_hip(hipError_t e, const char *what) { return hip_fail(e, what); }
+int require_device() { return ensure_device(); }
+}  // namespace yh
 
 extern "C" {
 

@@ -1,0 +1,152 @@
+// Row operators in 8 bits: declarations shared by their kernels and their C-ABI layer, and the device
+// helpers for rows of float32 / bfloat16 / float16 whose length and pitch are arbitrary.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "yolohead.h"
+
+namespace yh {
+
+// yh_abi.hip: stores the thread's error message and returns `code`; looks for a HIP device.
+int report(int code, const char *fmt, ...);
+int report_hip(hipError_t e, const char *what);
+int require_device();
+
+// ---- what the launchers take --------------------------------------------
+struct Rows {            // a matrix of rows: `ld` elements from one row to the next
+    const void *p;
+    int64_t ld;
+    int32_t type;        // yh_dtype
+};
+
+hipError_t launch_quantize(const Rows &x, int64_t rows, int32_t cols, int8_t *codes, int64_t ldc, float *scale, hipStream_t st);
+hipError_t launch_dequantize(const int8_t *codes, int64_t ldc, const float *scale, int64_t rows, int32_t cols,
+                             void *out, int64_t ldo, int32_t type, hipStream_t st);
+
+int norm_blocks(int64_t rows, int32_t cols, int32_t type);      // blocks per channel slab of the reductions
+hipError_t launch_norm_forward(const Rows &z, const Rows &res, int64_t rows, int32_t cols, const float *gamma, const float *beta,
+                               double eps, float slope, void *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale,
+                               float *mean, float *invstd, float *running_mean, float *running_var, double momentum,
+                               void *workspace, hipStream_t st);
+hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, const int8_t *kept, int64_t ldk, const float *scale,
+                                const float *gamma, const float *invstd, float slope, void *dz, int64_t lddz,
+                                float *dgamma, float *dbeta, void *workspace, hipStream_t st);
+
+hipError_t launch_int8_product(const int8_t *x, int64_t ldx, const float *x_scale, int64_t rows, int32_t k,
+                               const int8_t *w, int64_t ldw, const float *w_scale, int32_t n, const float *bias,
+                               void *y, int64_t ldy, int32_t type, hipStream_t st);
+
+int weight_grad_chunks(int64_t rows, int32_t n, int32_t k);     // pieces the rows are cut into
+hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, const float *scale, int64_t rows,
+                              int32_t n, int32_t k, float *dw, float *db, void *workspace, hipStream_t st);
+hipError_t launch_input_grad(const Rows &dy, const int8_t *w, int64_t ldw, const float *w_scale, int64_t rows,
+                             int32_t n, int32_t k, void *dx, int64_t lddx, int32_t type, hipStream_t st);
+
+// ---- device helpers ------------------------------------------------------
+constexpr float kRowMin = 0x1p-110f;      // a row whose largest value is below this is zero: its scale stays a normal number
+constexpr int kCodeMax = 127;             // row codes: -127 .. 127
+constexpr int kKeptMax = 63;              // norm checkpoint: seven bits beside the sign of the activation's input
+
+template <class T> struct RowVec { static constexpr int V = 16 / (int)sizeof(T); };   // elements of a 16-byte access
+
+// Vectors that may stand at any element (global memory on gfx950 takes unaligned accesses).  As vector types they stay
+// one access each: an element-wise copy is taken apart and partly shared with the code for a row's end.
+template <class T, int V> struct Loose { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)), may_alias)); };
+template <int B> struct LooseBytes { typedef uint32_t type __attribute__((ext_vector_type(B / 4), aligned(1), may_alias)); };
+template <> struct LooseBytes<4> { typedef uint32_t type __attribute__((aligned(1), may_alias)); };
+
+// `left` elements of a row from p on, as float32; what lies behind the row's end is not read and comes back zero.
+// The address is aligned to an element only: rows of odd length start anywhere.
+template <class T, int V>
+__device__ __forceinline__ void load_vec(float (&out)[V], const T *p, int left)
+{
+    if (left >= V) {
+        const typename Loose<T, V>::type t = *reinterpret_cast<const typename Loose<T, V>::type *>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = (float)t[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = i < left ? (float)p[i] : 0.0f;
+    }
+}
+
+// One rounding, to nearest even, of a float32 result to the row's type.
+template <class T, int V>
+__device__ __forceinline__ void store_vec(T *p, const float (&v)[V], int left)
+{
+    if (left >= V) {
+        typename Loose<T, V>::type t;
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = (T)v[i];
+        *reinterpret_cast<typename Loose<T, V>::type *>(p) = t;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) p[i] = (T)v[i];
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void store_bytes(int8_t *p, const uint32_t (&w)[V / 4], int left)
+{
+    if (left >= V) {
+        typename LooseBytes<V>::type t;
+        __builtin_memcpy(&t, w, V);
+        *reinterpret_cast<typename LooseBytes<V>::type *>(p) = t;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) p[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void load_bytes(uint32_t (&w)[V / 4], const int8_t *p, int left)
+{
+    if (left >= V) {
+        const typename LooseBytes<V>::type t = *reinterpret_cast<const typename LooseBytes<V>::type *>(p);
+        __builtin_memcpy(w, &t, V);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
+    }
+}
+
+__device__ __forceinline__ float code_value(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
+
+// Round-half-even of the exact product x * r, |x * r| <= 127.0001: the fused multiply-add rounds once, to the unit of
+// 1.5 * 2^23, so the whole number sits in the sum's low byte as two's complement.
+__device__ __forceinline__ uint32_t code_bits(float x, float r) { return __float_as_uint(__builtin_fmaf(x, r, 12582912.0f)); }
+
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    // v_perm_b32: bytes 0..3 are the second operand's, 4..7 the first's
+    const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+    return lo | hi;
+}
+
+// Largest |value| bits of a row, over the `lanes` (a power of two) neighbouring lanes that hold it.  Magnitudes are
+// compared as integers: every NaN is above infinity, infinity above every number.
+__device__ __forceinline__ uint32_t row_max(uint32_t m, int lanes)
+{
+    for (int o = 1; o < lanes; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+    return m;
+}
+
+struct RowScale { float r, s; bool live; };
+// r = levels / max, s = max / levels.  A row with an infinity or a NaN gets the scale NaN, so that everything computed
+// from it is NaN; a row that is zero (or below kRowMin) the scale 0; both have codes 0.
+__device__ __forceinline__ RowScale row_scale(uint32_t m, float levels)
+{
+    const float top = __uint_as_float(m);
+    RowScale k;
+    k.live = m < 0x7f800000u && top >= kRowMin;
+    k.r = k.live ? levels / top : 0.0f;
+    k.s = k.live ? top / levels : (m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : 0.0f);
+    return k;
+}
+
+}  // namespace yh

@@ -1,0 +1,575 @@
+// Row operators bound by memory: row codes (write and read) and batch normalisation with leaky ReLU on an 8-bit
+// checkpoint, forward and backward.
+#include <algorithm>
+#include "yh_rows.h"
+
+namespace yh {
+namespace {
+
+constexpr int kThreads = 256;
+
+int pow2_at_least(int v)
+{
+    int p = 1;
+    while (p < v) p <<= 1;
+    return p;
+}
+
+// How a wavefront holds rows in registers: `lanes` neighbouring lanes a row, each with `vecs` vectors of V elements,
+// `lanes` vectors apart.  Four vectors a lane keep 4 KiB of loads in flight a wavefront; rows shorter than that share
+// the wavefront, with at least eight lanes (128 contiguous bytes) each.
+struct RowPlan { int lanes, vecs; };
+RowPlan plan_row(int cols, int V)
+{
+    const int nv = (cols + V - 1) / V;
+    RowPlan p;
+    p.lanes = std::min(64, std::max(std::min(8, pow2_at_least(nv)), pow2_at_least((nv + 3) / 4)));
+    p.vecs = (nv + p.lanes - 1) / p.lanes;
+    return p;
+}
+
+template <class T, int IT>
+__global__ __launch_bounds__(kThreads) void k_quantize(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *codes, int64_t ldc,
+                                                       float *scale, int lanes)
+{
+    constexpr int V = RowVec<T>::V;
+    const int lane = threadIdx.x & 63, sub = lane & (lanes - 1);
+    const int64_t wave = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    const int64_t row = wave * (64 / lanes) + lane / lanes;
+    float v[IT][V];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int c = (i * lanes + sub) * V;
+        load_vec<T, V>(v[i], x + row * ldx + c, row < rows ? cols - c : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
+    const RowScale k = row_scale(row_max(m, lanes), (float)kCodeMax);
+    if (row >= rows) return;
+    if (sub == 0) scale[row] = k.s;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int c = (i * lanes + sub) * V;
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const uint32_t q = pack4(code_bits(v[i][j], k.r), code_bits(v[i][j + 1], k.r), code_bits(v[i][j + 2], k.r), code_bits(v[i][j + 3], k.r));
+            w[j / 4] = k.live ? q : 0u;
+        }
+        store_bytes<V>(codes + row * ldc + c, w, cols - c);
+    }
+}
+
+// The largest of a workgroup's values; `top`: one word a wavefront, free again when the call returns everywhere.
+__device__ __forceinline__ uint32_t workgroup_max(uint32_t m, uint32_t *top)
+{
+    m = row_max(m, 64);
+    __syncthreads();                                 // the last call's words have been read
+    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) m = max(m, top[i]);
+    return m;
+}
+
+// Rows longer than the registers of a wavefront: a workgroup a row, read twice (the second time from the caches).
+template <class T>
+__global__ __launch_bounds__(kThreads) void k_quantize_long(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *codes, int64_t ldc, float *scale)
+{
+    constexpr int V = RowVec<T>::V;
+    __shared__ uint32_t top[kThreads / 64];
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *p = x + row * ldx;
+        uint32_t m = 0;
+        for (int c = threadIdx.x * V; c < cols; c += kThreads * V) {
+            float v[V];
+            load_vec<T, V>(v, p + c, cols - c);
+#pragma unroll
+            for (int j = 0; j < V; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        }
+        m = workgroup_max(m, top);
+        const RowScale k = row_scale(m, (float)kCodeMax);
+        if (threadIdx.x == 0) scale[row] = k.s;
+        for (int c = threadIdx.x * V; c < cols; c += kThreads * V) {
+            float v[V];
+            load_vec<T, V>(v, p + c, cols - c);
+            uint32_t w[V / 4];
+#pragma unroll
+            for (int j = 0; j < V; j += 4) {
+                const uint32_t q = pack4(code_bits(v[j], k.r), code_bits(v[j + 1], k.r), code_bits(v[j + 2], k.r), code_bits(v[j + 3], k.r));
+                w[j / 4] = k.live ? q : 0u;
+            }
+            store_bytes<V>(codes + row * ldc + c, w, cols - c);
+        }
+    }
+}
+
+template <class T, int IT>
+__global__ __launch_bounds__(kThreads) void k_dequantize(const int8_t *codes, int64_t ldc, const float *scale, int64_t rows, int cols,
+                                                         T *out, int64_t ldo, int lanes)
+{
+    constexpr int V = RowVec<T>::V;
+    const int lane = threadIdx.x & 63, sub = lane & (lanes - 1);
+    const int64_t wave = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    const int64_t row = wave * (64 / lanes) + lane / lanes;
+    if (row >= rows) return;
+    const float s = scale[row];
+    for (int base = 0; base < cols; base += IT * lanes * V) {
+        uint32_t w[IT][V / 4];
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = base + (i * lanes + sub) * V;
+            load_bytes<V>(w[i], codes + row * ldc + c, cols - c);
+        }
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = base + (i * lanes + sub) * V;
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = code_value(w[i][j / 4], j % 4) * s;
+            store_vec<T, V>(out + row * ldo + c, v, cols - c);
+        }
+    }
+}
+
+// ---- batch normalisation + leaky ReLU (+ shortcut) on an 8-bit checkpoint ----
+// Forward, per channel c over all rows:  mean = sum z / M, var = sum (z - mean)^2 / M, both in 64 bits (the differences to
+// the channel's first value are exact there, so neither a large mean nor many rows cost anything), then rounded once:
+// mean, invstd = 1 / sqrt(var + eps) in float32.  Per element in float32, each operation rounded by itself:
+//   xhat = (z - mean) * invstd,  u = xhat * gamma + beta,  a = (u > 0 ? u : slope * u) [+ residual].
+// The checkpoint is one byte an element: the sign of u in the lowest bit, exactly as the forward pass decided it, and
+// xhat in seven bits above it, relative to the row's largest |xhat| / 63.  The backward pass needs the sign for every
+// element's gradient and xhat only for a sum over the rows (dgamma) and for that sum's small share of each element, where
+// the rounding of the code averages out; eight bits for xhat and the sign taken from them would be off on the elements
+// next to zero.
+// Backward:  du = sign ? da : slope * da,  dbeta = sum du,  dgamma = sum du * xq,
+//            dz = gamma * invstd * (du - dbeta / M - xq * dgamma / M).
+// Both directions read their input twice, with the per-channel sums in between: a reduction into one partial pair a
+// workgroup and channel, a small launch that adds the partials in a fixed order, and an elementwise pass.
+
+// A workgroup's threads over (channel vectors, rows) in the reductions.
+struct ReducePlan { int tx, ty, slabs, blocks; int64_t rows_per_block; };
+ReducePlan plan_reduce(int64_t rows, int cols, int V)
+{
+    const int cv = (cols + V - 1) / V;
+    ReducePlan p;
+    p.tx = std::min(64, pow2_at_least(cv));
+    p.ty = kThreads / p.tx;
+    p.slabs = (cv + p.tx - 1) / p.tx;
+    // about 1024 workgroups in all (four a compute unit), each thread with at least eight rows
+    const int64_t by_rows = (rows + p.ty * 8 - 1) / ((int64_t)p.ty * 8);
+    const int64_t want = std::max(1, 1024 / p.slabs);
+    const int64_t blocks = std::max<int64_t>(1, std::min(want, by_rows));
+    p.rows_per_block = (rows + blocks - 1) / blocks;
+    p.blocks = (int)((rows + p.rows_per_block - 1) / p.rows_per_block);
+    return p;
+}
+
+// Adds the threads' pairs over ty and writes the workgroup's pair of each channel: part[2][cols][blocks].
+template <int V>
+__device__ __forceinline__ void reduce_pairs(double (&s1)[V], double (&s2)[V], int tx, int ty, int TX, int cvec, int cols, double *part, int blocks)
+{
+    __shared__ double buf[kThreads * V];
+    for (int which = 0; which < 2; ++which) {
+        double (&s)[V] = which ? s2 : s1;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < V; ++j) buf[j * kThreads + threadIdx.x] = s[j];
+        for (int half = kThreads / 2; half >= TX; half >>= 1) {
+            __syncthreads();
+            if ((int)threadIdx.x < half)
+#pragma unroll
+                for (int j = 0; j < V; ++j) buf[j * kThreads + threadIdx.x] += buf[j * kThreads + threadIdx.x + half];
+        }
+        if (ty == 0)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int c = cvec * V + j;
+                if (c < cols) part[((int64_t)which * cols + c) * blocks + blockIdx.x] = buf[j * kThreads + tx];
+            }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int TX, int64_t rows_per_block, double *part)
+{
+    constexpr int V = RowVec<T>::V, U = 4;
+    const int tx = threadIdx.x & (TX - 1), ty = threadIdx.x / TX, TY = kThreads / TX;
+    const int cvec = blockIdx.y * TX + tx, c = cvec * V, left = cols - c;
+    const int64_t r0 = (int64_t)blockIdx.x * rows_per_block, r1 = min(rows, r0 + rows_per_block);
+    double s1[V], s2[V];
+    float first[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
+    load_vec<T, V>(first, z + c, left);
+    const T *p = z + c;
+    for (int64_t r = r0 + ty; r < r1; r += (int64_t)U * TY) {
+        float v[U][V];
+#pragma unroll
+        for (int i = 0; i < U; ++i) load_vec<T, V>(v[i], p + (r + i * TY) * ldz, r + i * TY < r1 ? left : 0);
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (r + i * TY < r1)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const double d = (double)v[i][j] - (double)first[j];
+                    s1[j] += d;
+                    s2[j] = __builtin_fma(d, d, s2[j]);
+                }
+    }
+    reduce_pairs<V>(s1, s2, tx, ty, TX, cvec, cols, part, gridDim.x);
+}
+
+// One wavefront a channel: the partials in a fixed order, whatever ran first.
+__device__ __forceinline__ double sum_partials(const double *p, int blocks, int lane)
+{
+    double s = 0.0;
+    for (int i = lane; i < blocks; i += 64) s += p[i];
+    for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
+    return s;
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads) void k_norm_stats_finish(const double *part, int blocks, const T *z, int64_t rows, int cols, double eps,
+                                                                float *mean, float *invstd, float *running_mean, float *running_var, double momentum)
+{
+    const int c = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (c >= cols) return;
+    const double m = (double)rows;
+    const double d = sum_partials(part + (int64_t)c * blocks, blocks, lane) / m;
+    const double e = sum_partials(part + ((int64_t)cols + c) * blocks, blocks, lane) / m;
+    if (lane) return;
+    const double mu = (double)(float)z[c] + d;
+    double var = e - d * d;
+    if (var < 0.0) var = 0.0;                        // a NaN stays one
+    mean[c] = (float)mu;
+    invstd[c] = (float)(1.0 / sqrt(var + eps));
+    if (running_mean) {
+        running_mean[c] = (float)((1.0 - momentum) * (double)running_mean[c] + momentum * mu);
+        running_var[c] = (float)((1.0 - momentum) * (double)running_var[c] + momentum * (rows > 1 ? var * (m / (m - 1.0)) : var));
+    }
+}
+
+template <class T, int IT>
+__global__ __launch_bounds__(kThreads) void k_norm_apply(const T *z, int64_t ldz, const T *res, int64_t ldr, int64_t rows, int cols,
+                                                         const float *mean, const float *invstd, const float *gamma, const float *beta, float slope,
+                                                         T *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale, int lanes, int64_t waves)
+{
+    constexpr int V = RowVec<T>::V;
+    const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), rpw = 64 / lanes;
+    float mu[IT][V], is[IT][V], ga[IT][V], be[IT][V];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int c = (i * lanes + sub) * V;
+        load_vec<float, V>(mu[i], mean + c, cols - c);
+        load_vec<float, V>(is[i], invstd + c, cols - c);
+        load_vec<float, V>(ga[i], gamma + c, cols - c);
+        load_vec<float, V>(be[i], beta + c, cols - c);
+    }
+    // every lane of a wavefront takes part in the row maximum: the loop's bound is the wavefront's first row
+    for (int64_t g = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); g * rpw < rows; g += waves) {
+        const int64_t row = g * rpw + lane / lanes;
+        const bool in = row < rows;
+        float v[IT][V], rs[IT][V];
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = (i * lanes + sub) * V;
+            load_vec<T, V>(v[i], z + row * ldz + c, in ? cols - c : 0);
+            if (res) load_vec<T, V>(rs[i], res + row * ldr + c, in ? cols - c : 0);
+        }
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int c = (i * lanes + sub) * V + j;
+                v[i][j] = (v[i][j] - mu[i][j]) * is[i][j];
+                if (c < cols) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
+            }
+        const RowScale k = row_scale(row_max(m, lanes), (float)kKeptMax);
+        if (!in) continue;
+        if (kept && sub == 0) scale[row] = k.s;
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = (i * lanes + sub) * V;
+            uint32_t w[V / 4], b[V];
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float u = v[i][j] * ga[i][j] + be[i][j];
+                const bool up = u > 0.0f;
+                o[j] = up ? u : slope * u;
+                if (res) o[j] += rs[i][j];
+                const uint32_t q = k.live ? code_bits(v[i][j], k.r) : 0u;
+                b[j] = (q << 1) | (up ? 1u : 0u);
+            }
+            store_vec<T, V>(a + row * lda + c, o, cols - c);
+            if (kept) {
+#pragma unroll
+                for (int j = 0; j < V; j += 4) w[j / 4] = pack4(b[j], b[j + 1], b[j + 2], b[j + 3]);
+                store_bytes<V>(kept + row * ldk + c, w, cols - c);
+            }
+        }
+    }
+}
+
+// Rows longer than a wavefront's registers: a workgroup a row, read twice.
+template <class T>
+__global__ __launch_bounds__(kThreads) void k_norm_apply_long(const T *z, int64_t ldz, const T *res, int64_t ldr, int64_t rows, int cols,
+                                                              const float *mean, const float *invstd, const float *gamma, const float *beta, float slope,
+                                                              T *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale)
+{
+    constexpr int V = RowVec<T>::V;
+    __shared__ uint32_t top[kThreads / 64];
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        uint32_t m = 0;
+        for (int c = threadIdx.x * V; c < cols; c += kThreads * V) {
+            float v[V], mu[V], is[V];
+            load_vec<T, V>(v, z + row * ldz + c, cols - c);
+            load_vec<float, V>(mu, mean + c, cols - c);
+            load_vec<float, V>(is, invstd + c, cols - c);
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (c + j < cols) m = max(m, __float_as_uint((v[j] - mu[j]) * is[j]) & 0x7fffffffu);
+        }
+        m = workgroup_max(m, top);
+        const RowScale k = row_scale(m, (float)kKeptMax);
+        if (kept && threadIdx.x == 0) scale[row] = k.s;
+        for (int c = threadIdx.x * V; c < cols; c += kThreads * V) {
+            float v[V], rs[V], mu[V], is[V], ga[V], be[V], o[V];
+            uint32_t w[V / 4], b[V];
+            load_vec<T, V>(v, z + row * ldz + c, cols - c);
+            if (res) load_vec<T, V>(rs, res + row * ldr + c, cols - c);
+            load_vec<float, V>(mu, mean + c, cols - c);
+            load_vec<float, V>(is, invstd + c, cols - c);
+            load_vec<float, V>(ga, gamma + c, cols - c);
+            load_vec<float, V>(be, beta + c, cols - c);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xh = (v[j] - mu[j]) * is[j], u = xh * ga[j] + be[j];
+                const bool up = u > 0.0f;
+                o[j] = up ? u : slope * u;
+                if (res) o[j] += rs[j];
+                b[j] = ((k.live ? code_bits(xh, k.r) : 0u) << 1) | (up ? 1u : 0u);
+            }
+            store_vec<T, V>(a + row * lda + c, o, cols - c);
+            if (kept) {
+#pragma unroll
+                for (int j = 0; j < V; j += 4) w[j / 4] = pack4(b[j], b[j + 1], b[j + 2], b[j + 3]);
+                store_bytes<V>(kept + row * ldk + c, w, cols - c);
+            }
+        }
+    }
+}
+
+// The checkpoint's byte: xhat's code and the activation's side.
+__device__ __forceinline__ float kept_code(uint32_t w, int i) { return (float)((int8_t)(w >> (8 * i)) >> 1); }
+__device__ __forceinline__ bool kept_side(uint32_t w, int i) { return (w >> (8 * i)) & 1u; }
+
+template <class T>
+__global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
+                                                             int64_t rows, int cols, float slope, int TX, int64_t rows_per_block, double *part)
+{
+    constexpr int V = RowVec<T>::V, U = 4;
+    const int tx = threadIdx.x & (TX - 1), ty = threadIdx.x / TX, TY = kThreads / TX;
+    const int cvec = blockIdx.y * TX + tx, c = cvec * V, left = cols - c;
+    const int64_t r0 = (int64_t)blockIdx.x * rows_per_block, r1 = min(rows, r0 + rows_per_block);
+    double s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
+    for (int64_t r = r0 + ty; r < r1; r += (int64_t)U * TY) {
+        float v[U][V], s[U];
+        uint32_t w[U][V / 4];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int64_t rr = r + i * TY;
+            const int l = rr < r1 ? left : 0;
+            load_vec<T, V>(v[i], da + rr * ldd + c, l);
+            load_bytes<V>(w[i], kept + rr * ldk + c, l);
+            s[i] = rr < r1 ? scale[rr] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float du = kept_side(w[i][j / 4], j % 4) ? v[i][j] : slope * v[i][j];
+                const float xq = kept_code(w[i][j / 4], j % 4) * s[i];
+                s1[j] += (double)du;
+                s2[j] = __builtin_fma((double)du, (double)xq, s2[j]);
+            }
+    }
+    reduce_pairs<V>(s1, s2, tx, ty, TX, cvec, cols, part, gridDim.x);
+}
+
+__global__ __launch_bounds__(kThreads) void k_norm_grad_finish(const double *part, int blocks, int64_t rows, int cols, const float *gamma, const float *invstd,
+                                                               float *dgamma, float *dbeta, float *coef)
+{
+    const int c = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (c >= cols) return;
+    const double b = sum_partials(part + (int64_t)c * blocks, blocks, lane);
+    const double g = sum_partials(part + ((int64_t)cols + c) * blocks, blocks, lane);
+    if (lane) return;
+    dbeta[c] = (float)b;
+    dgamma[c] = (float)g;
+    coef[c] = gamma[c] * invstd[c];
+    coef[cols + c] = (float)(b / (double)rows);
+    coef[2 * (int64_t)cols + c] = (float)(g / (double)rows);
+}
+
+template <class T, int IT>
+__global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
+                                                              int64_t rows, int cols, float slope, const float *coef, T *dz, int64_t ldz, int lanes, int64_t waves)
+{
+    constexpr int V = RowVec<T>::V;
+    const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), rpw = 64 / lanes;
+    const int c0 = blockIdx.y * IT * lanes * V;
+    float g[IT][V], cb[IT][V], cg[IT][V];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int c = c0 + (i * lanes + sub) * V;
+        load_vec<float, V>(g[i], coef + c, cols - c);
+        load_vec<float, V>(cb[i], coef + cols + c, cols - c);
+        load_vec<float, V>(cg[i], coef + 2 * (int64_t)cols + c, cols - c);
+    }
+    for (int64_t w0 = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); w0 * rpw < rows; w0 += waves) {
+        const int64_t row = w0 * rpw + lane / lanes;
+        if (row >= rows) continue;
+        float v[IT][V];
+        uint32_t w[IT][V / 4];
+        const float s = scale[row];
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = c0 + (i * lanes + sub) * V;
+            load_vec<T, V>(v[i], da + row * ldd + c, cols - c);
+            load_bytes<V>(w[i], kept + row * ldk + c, cols - c);
+        }
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = c0 + (i * lanes + sub) * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float du = kept_side(w[i][j / 4], j % 4) ? v[i][j] : slope * v[i][j];
+                const float xq = kept_code(w[i][j / 4], j % 4) * s;
+                v[i][j] = g[i][j] * (du - cb[i][j] - xq * cg[i][j]);
+            }
+            store_vec<T, V>(dz + row * ldz + c, v[i], cols - c);
+        }
+    }
+}
+
+// Calls f(T()) with the C++ type of a yh_dtype.
+template <class F>
+void with_type(int32_t type, F f)
+{
+    if (type == YH_FLOAT32) f(float());
+    else if (type == YH_BFLOAT16) f((__bf16)0.0f);
+    else f((_Float16)0.0f);
+}
+
+// Calls f.template operator()<IT>() is not available before C++20: the vector counts are spelled out.
+#define YH_WITH_VECS(vecs, CALL)            \
+    do {                                    \
+        if ((vecs) <= 1) { CALL(1); }       \
+        else if ((vecs) <= 2) { CALL(2); }  \
+        else if ((vecs) <= 4) { CALL(4); }  \
+        else { CALL(6); }                   \
+    } while (0)
+
+unsigned row_blocks(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 1 << 20); }
+unsigned waves_to_blocks(int64_t waves) { return (unsigned)((waves + kThreads / 64 - 1) / (kThreads / 64)); }
+
+}  // namespace
+
+hipError_t launch_quantize(const Rows &x, int64_t rows, int32_t cols, int8_t *codes, int64_t ldc, float *scale, hipStream_t st)
+{
+    with_type(x.type, [&](auto t) {
+        using T = decltype(t);
+        const T *p = static_cast<const T *>(x.p);
+        const RowPlan r = plan_row(cols, RowVec<T>::V);
+        if (r.vecs > 6) {
+            k_quantize_long<T><<<dim3(row_blocks(rows)), kThreads, 0, st>>>(p, rows, cols, x.ld, codes, ldc, scale);
+            return;
+        }
+        const unsigned blocks = waves_to_blocks((rows * r.lanes + 63) / 64);
+#define CALL(IT) k_quantize<T, IT><<<dim3(blocks), kThreads, 0, st>>>(p, rows, cols, x.ld, codes, ldc, scale, r.lanes)
+        YH_WITH_VECS(r.vecs, CALL);
+#undef CALL
+    });
+    return hipGetLastError();
+}
+
+hipError_t launch_dequantize(const int8_t *codes, int64_t ldc, const float *scale, int64_t rows, int32_t cols,
+                             void *out, int64_t ldo, int32_t type, hipStream_t st)
+{
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        const RowPlan r = plan_row(cols, RowVec<T>::V);
+        const unsigned blocks = waves_to_blocks((rows * r.lanes + 63) / 64);
+#define CALL(IT) k_dequantize<T, IT><<<dim3(blocks), kThreads, 0, st>>>(codes, ldc, scale, rows, cols, static_cast<T *>(out), ldo, r.lanes)
+        YH_WITH_VECS(r.vecs, CALL);
+#undef CALL
+    });
+    return hipGetLastError();
+}
+
+int norm_blocks(int64_t rows, int32_t cols, int32_t type)
+{
+    return plan_reduce(rows, cols, type == YH_FLOAT32 ? RowVec<float>::V : RowVec<__bf16>::V).blocks;
+}
+
+hipError_t launch_norm_forward(const Rows &z, const Rows &res, int64_t rows, int32_t cols, const float *gamma, const float *beta,
+                               double eps, float slope, void *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale,
+                               float *mean, float *invstd, float *running_mean, float *running_var, double momentum,
+                               void *workspace, hipStream_t st)
+{
+    double *part = static_cast<double *>(workspace);
+    with_type(z.type, [&](auto t) {
+        using T = decltype(t);
+        const T *p = static_cast<const T *>(z.p), *q = static_cast<const T *>(res.p);
+        const ReducePlan d = plan_reduce(rows, cols, RowVec<T>::V);
+        k_norm_stats<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, rows, cols, z.ld, d.tx, d.rows_per_block, part);
+        k_norm_stats_finish<T><<<dim3(waves_to_blocks(cols)), kThreads, 0, st>>>(part, d.blocks, p, rows, cols, eps, mean, invstd, running_mean, running_var, momentum);
+        const RowPlan r = plan_row(cols, RowVec<T>::V);
+        if (r.vecs > 6) {
+            k_norm_apply_long<T><<<dim3(row_blocks(rows)), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope,
+                                                                            static_cast<T *>(a), lda, kept, ldk, scale);
+            return;
+        }
+        const unsigned blocks = std::min(2048u, waves_to_blocks((rows * r.lanes + 63) / 64));
+#define CALL(IT) k_norm_apply<T, IT><<<dim3(blocks), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope, \
+                                                                        static_cast<T *>(a), lda, kept, ldk, scale, r.lanes, (int64_t)blocks * (kThreads / 64))
+        YH_WITH_VECS(r.vecs, CALL);
+#undef CALL
+    });
+    return hipGetLastError();
+}
+
+hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, const int8_t *kept, int64_t ldk, const float *scale,
+                                const float *gamma, const float *invstd, float slope, void *dz, int64_t lddz,
+                                float *dgamma, float *dbeta, void *workspace, hipStream_t st)
+{
+    double *part = static_cast<double *>(workspace);
+    with_type(da.type, [&](auto t) {
+        using T = decltype(t);
+        const T *p = static_cast<const T *>(da.p);
+        const ReducePlan d = plan_reduce(rows, cols, RowVec<T>::V);
+        float *coef = reinterpret_cast<float *>(part + 2 * (int64_t)cols * d.blocks);
+        k_norm_grad_sums<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, da.ld, kept, ldk, scale, rows, cols, slope, d.tx, d.rows_per_block, part);
+        k_norm_grad_finish<<<dim3(waves_to_blocks(cols)), kThreads, 0, st>>>(part, d.blocks, rows, cols, gamma, invstd, dgamma, dbeta, coef);
+        const RowPlan r = plan_row(cols, RowVec<T>::V);
+        const int vecs = std::min(4, r.vecs), step = (vecs <= 1 ? 1 : vecs <= 2 ? 2 : 4) * r.lanes * RowVec<T>::V;
+        const unsigned blocks = std::min(2048u, waves_to_blocks((rows * r.lanes + 63) / 64));
+#define CALL(IT) k_norm_grad_apply<T, IT><<<dim3(blocks, (cols + step - 1) / step), kThreads, 0, st>>>( \
+            p, da.ld, kept, ldk, scale, rows, cols, slope, coef, static_cast<T *>(dz), lddz, r.lanes, (int64_t)blocks * (kThreads / 64))
+        if (vecs <= 1) CALL(1);
+        else if (vecs <= 2) CALL(2);
+        else CALL(4);
+#undef CALL
+    });
+    return hipGetLastError();
+}
+
+}  // namespace yh

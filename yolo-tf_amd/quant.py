@@ -1,0 +1,264 @@
+"""Row operators in 8 bits for the convolution stacks: activation checkpoints, the
+pointwise (1x1) convolution in 8-bit integers with its gradients, and batch
+normalisation with leaky ReLU on an 8-bit checkpoint (kernels: csrc/yh_rows.hip,
+csrc/yh_product.hip; declarations and definitions: include/yolohead.h).
+
+A "row" is one pixel: tensors are [..., channels] in float32, bfloat16 or float16
+on a HIP device, NHWC for an activation; leading dimensions that have one stride
+between them (a channel slice of a wider tensor, say) are read in place, others are
+copied first.  Calls go to the current stream of the tensors' device; outputs and
+scratch come from torch's allocator, so a call can be captured into a graph.  There
+is no CPU path: without a HIP device these functions raise.
+
+The functions of the first half compute; the second half binds them to autograd, for
+backbone.ConvBN (`pointwise='int8'`, `checkpoints='int8'`).  Their gradients take
+the roundings for the identity (straight through) and cannot be differentiated
+again."""
+import ctypes
+
+import torch
+import torch.nn.functional as F
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _abi
+
+_TYPES = {torch.float32: _abi.YH_FLOAT32, torch.bfloat16: _abi.YH_BFLOAT16, torch.float16: _abi.YH_FLOAT16}
+
+
+# ------------------------------------------------------------------ helpers
+def _device_of(x, what):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError('%s must be a torch tensor on a HIP device' % what)
+    if x.device.type != 'cuda':
+        raise RuntimeError('%s must live on a HIP device (got %s); there is no CPU path' % (what, x.device))
+    return x.device
+
+
+def _float_type(x, what):
+    code = _TYPES.get(x.dtype)
+    if code is None:
+        raise ValueError('%s must be float32, bfloat16 or float16, got %s' % (what, x.dtype))
+    return code
+
+
+def _rows(x, what):
+    """x as [rows, channels] with adjacent channels: (tensor that owns the memory, rows, channels, elements between rows)."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError('%s must be [..., channels] with at least one channel, got %s' % (what, tuple(x.shape)))
+    x = x.detach()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    rows, cols = x.shape
+    return x, rows, cols, x.stride(0) if rows > 1 else cols
+
+
+def _vector(v, n, dev, what):
+    """A float32 vector of n adjacent values on `dev`."""
+    if not isinstance(v, torch.Tensor) or v.dtype != torch.float32 or v.device != dev or v.numel() != n:
+        raise ValueError('%s must be %d float32 values on %s' % (what, n, dev))
+    v = v.detach()
+    return v if v.is_contiguous() else v.contiguous()
+
+
+def _codes(q, dev, what):
+    if not isinstance(q, torch.Tensor) or q.dtype != torch.int8 or q.device != dev:
+        raise ValueError('%s must be int8 codes on %s' % (what, dev))
+    return _rows(q, what)
+
+
+def _new_codes(shape, dev):
+    """int8 codes of `shape` whose rows start at multiples of 16 bytes: a view of a wider buffer where needed."""
+    cols = shape[-1]
+    wide = (cols + 15) // 16 * 16
+    if wide == cols:
+        return torch.empty(shape, dtype=torch.int8, device=dev), cols
+    return torch.empty(tuple(shape[:-1]) + (wide,), dtype=torch.int8, device=dev)[..., :cols], wide
+
+
+def _call(dev, fn, *args):
+    """One library call on `dev`'s current stream."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        _abi.check(fn(*args, stream))
+    else:
+        with torch.cuda.device(dev):
+            _abi.check(fn(*args, stream))
+
+
+def _scratch(size_fn, dev, *sizes):
+    """(pointer, bytes, tensor that keeps it) of a workspace for one call."""
+    n = ctypes.c_size_t(0)
+    _abi.check(size_fn(*sizes, ctypes.byref(n)))
+    if n.value == 0:
+        return None, 0, None
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    return ws.data_ptr(), n.value, ws
+
+
+# ------------------------------------------------------------------ row codes
+def quantize_rows(x):
+    """(codes int8 shaped like x, scale float32 [...]) of the rows of x: scale = max|x| / 127, code =
+    x / scale rounded.  A row of zeros has the scale 0; one with an infinity or a NaN the scale NaN."""
+    dev = _device_of(x, 'x')
+    kind = _float_type(x, 'x')
+    xr, rows, cols, ld = _rows(x, 'x')
+    codes, ldc = _new_codes(tuple(x.shape), dev)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    _call(dev, _abi.load().yh_quantize_rows, xr.data_ptr(), kind, ld, rows, cols, codes.data_ptr(), ldc, scale.data_ptr())
+    return codes, scale
+
+
+def dequantize_rows(codes, scale, dtype=torch.float32):
+    """The values that row codes stand for: codes * scale, in `dtype`."""
+    dev = _device_of(codes, 'codes')
+    qr, rows, cols, ld = _codes(codes, dev, 'codes')
+    scale = _vector(scale, rows, dev, 'scale')
+    x = torch.empty(codes.shape, dtype=dtype, device=dev)
+    _call(dev, _abi.load().yh_dequantize_rows, qr.data_ptr(), ld, scale.data_ptr(), rows, cols, x.data_ptr(),
+          _float_type(x, 'dtype'), cols)
+    return x
+
+
+# ------------------------------------------------------------------ products
+def matmul_int8(x, w_codes, w_scale, bias=None, x_scale=None, out_dtype=None, want_codes=False):
+    """A pointwise convolution in 8-bit integers: x [..., K] times the rows of w_codes [N, K], scaled by each
+    row's and each output channel's scale, plus bias [N]: [..., N] in out_dtype (default: x's type).
+    x: float rows, whose codes are taken within the call; or int8 codes with x_scale [...] (out_dtype then
+    defaults to float32).  w_codes, w_scale: quantize_rows of the weights.  want_codes: returns
+    (y, codes, scale), the checkpoint that weight_grad reads."""
+    dev = _device_of(x, 'x')
+    lib = _abi.load()
+    xr, rows, k, ldx = _rows(x, 'x')
+    wr, n, wk, ldw = _codes(w_codes, dev, 'w_codes')
+    if w_codes.dim() != 2 or wk != k:
+        raise ValueError('w_codes must be [N, %d], got %s' % (k, tuple(w_codes.shape)))
+    w_scale = _vector(w_scale, n, dev, 'w_scale')
+    bias = None if bias is None else _vector(bias, n, dev, 'bias')
+    whole = x.dtype == torch.int8
+    if whole:
+        if x_scale is None or want_codes:
+            raise ValueError('int8 codes need x_scale, and are the codes already')
+        kind, x_scale = _abi.YH_INT8, _vector(x_scale, rows, dev, 'x_scale')
+        out_dtype = torch.float32 if out_dtype is None else out_dtype
+    else:
+        if x_scale is not None:
+            raise ValueError('x_scale belongs to int8 codes')
+        kind = _float_type(x, 'x')
+        out_dtype = x.dtype if out_dtype is None else out_dtype
+    y = torch.empty(tuple(x.shape[:-1]) + (n,), dtype=out_dtype, device=dev)
+    codes = scale = None
+    ldc = 0
+    if want_codes:
+        codes, ldc = _new_codes(tuple(x.shape), dev)
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    ws, nbytes, keep = _scratch(lib.yh_matmul_int8_workspace_bytes, dev, rows, k, n, kind, 1 if want_codes else 0)
+    _call(dev, lib.yh_matmul_int8, xr.data_ptr(), kind, ldx, x_scale.data_ptr() if whole else None, rows, k,
+          wr.data_ptr(), ldw, w_scale.data_ptr(), n, None if bias is None else bias.data_ptr(),
+          y.data_ptr(), _float_type(y, 'out_dtype'), n,
+          codes.data_ptr() if want_codes else None, ldc, scale.data_ptr() if want_codes else None, ws, nbytes)
+    return (y, codes, scale) if want_codes else y
+
+
+def weight_grad(dy, codes, scale, want_bias=False):
+    """dw [N, K] float32 = dy^T times the values of the row codes, from dy [..., N] and codes [..., K] with
+    scale [...]; with want_bias (dw, db [N]), db the sum of dy's rows."""
+    dev = _device_of(dy, 'dy')
+    lib = _abi.load()
+    kind = _float_type(dy, 'dy')
+    dr, rows, n, ldd = _rows(dy, 'dy')
+    qr, qrows, k, ldq = _codes(codes, dev, 'codes')
+    if qrows != rows:
+        raise ValueError('dy has %d rows, codes %d' % (rows, qrows))
+    scale = _vector(scale, rows, dev, 'scale')
+    dw = torch.empty((n, k), dtype=torch.float32, device=dev)
+    db = torch.empty((n,), dtype=torch.float32, device=dev) if want_bias else None
+    ws, nbytes, keep = _scratch(lib.yh_weight_grad_workspace_bytes, dev, rows, n, k)
+    _call(dev, lib.yh_weight_grad, dr.data_ptr(), kind, ldd, qr.data_ptr(), ldq, scale.data_ptr(), rows, n, k,
+          dw.data_ptr(), db.data_ptr() if want_bias else None, ws, nbytes)
+    return (dw, db) if want_bias else dw
+
+
+def input_grad(dy, w_codes, w_scale):
+    """dx [..., K] in dy's type = dy [..., N] times the values of the weight codes [N, K]."""
+    dev = _device_of(dy, 'dy')
+    kind = _float_type(dy, 'dy')
+    dr, rows, n, ldd = _rows(dy, 'dy')
+    wr, wn, k, ldw = _codes(w_codes, dev, 'w_codes')
+    if w_codes.dim() != 2 or wn != n:
+        raise ValueError('w_codes must be [%d, K], got %s' % (n, tuple(w_codes.shape)))
+    w_scale = _vector(w_scale, n, dev, 'w_scale')
+    dx = torch.empty(tuple(dy.shape[:-1]) + (k,), dtype=dy.dtype, device=dev)
+    _call(dev, _abi.load().yh_input_grad, dr.data_ptr(), kind, ldd, wr.data_ptr(), ldw, w_scale.data_ptr(), rows, n, k,
+          dx.data_ptr(), k)
+    return dx
+
+
+# ------------------------------------------------------------------ normalisation
+class NormKept:
+    """What norm_act leaves for norm_act_backward: `kept` int8 (the activation's side and xhat in seven bits) with
+    a scale for each row, mean and invstd [C] float32, and the call's gamma and slope."""
+
+    __slots__ = ('kept', 'scale', 'mean', 'invstd', 'gamma', 'slope')
+
+    def __init__(self, kept, scale, mean, invstd, gamma, slope):
+        self.kept, self.scale, self.mean, self.invstd, self.gamma, self.slope = kept, scale, mean, invstd, gamma, slope
+
+
+def norm_act(z, gamma, beta, eps, slope, residual=None, running=None, momentum=0.01, want_kept=True):
+    """Batch normalisation of z [..., C] on its own statistics, leaky ReLU of `slope` (1: none) and a shortcut:
+    (a shaped like z, NormKept), NormKept without its checkpoint if want_kept is False.
+    running: (mean, var) buffers [C], updated in place with `momentum` as torch.nn.BatchNorm2d does (one row
+    counts its variance as it is)."""
+    dev = _device_of(z, 'z')
+    lib = _abi.load()
+    kind = _float_type(z, 'z')
+    zr, rows, c, ldz = _rows(z, 'z')
+    gamma, beta = _vector(gamma, c, dev, 'gamma'), _vector(beta, c, dev, 'beta')
+    rr, ldr = None, 0
+    if residual is not None:
+        if not isinstance(residual, torch.Tensor) or residual.shape != z.shape or residual.dtype != z.dtype or residual.device != dev:
+            raise ValueError('residual must be %s in %s on %s' % (tuple(z.shape), z.dtype, dev))
+        rr, _, _, ldr = _rows(residual, 'residual')
+    rm = rv = None
+    if running is not None:
+        rm, rv = running
+        for t in (rm, rv):
+            if _vector(t, c, dev, 'running').data_ptr() != t.data_ptr():
+                raise ValueError('the running statistics must be contiguous: they are updated in place')
+    a = torch.empty(z.shape, dtype=z.dtype, device=dev)
+    kept = scale = None
+    ldk = 0
+    if want_kept:
+        kept, ldk = _new_codes(tuple(z.shape), dev)
+        scale = torch.empty(z.shape[:-1], dtype=torch.float32, device=dev)
+    stats = torch.empty((2, c), dtype=torch.float32, device=dev)
+    ws, nbytes, keep = _scratch(lib.yh_norm_act_workspace_bytes, dev, rows, c, kind)
+    _call(dev, lib.yh_norm_act_forward, zr.data_ptr(), ldz, None if rr is None else rr.data_ptr(), ldr, kind, rows, c,
+          gamma.data_ptr(), beta.data_ptr(), float(eps), float(slope), a.data_ptr(), c,
+          None if kept is None else kept.data_ptr(), ldk, None if scale is None else scale.data_ptr(),
+          stats.data_ptr(), stats.data_ptr() + 4 * c, None if rm is None else rm.data_ptr(),
+          None if rv is None else rv.data_ptr(), float(momentum), ws, nbytes)
+    return a, NormKept(kept, scale, stats[0], stats[1], gamma, float(slope))
+
+
+def norm_act_backward(da, kept):
+    """(dz, dgamma [C], dbeta [C]) of norm_act from a's gradient and the NormKept; the residual's gradient is da."""
+    dev = _device_of(da, 'da')
+    lib = _abi.load()
+    kind = _float_type(da, 'da')
+    if kept.kept is None:
+        raise ValueError('the forward call kept nothing (want_kept=False)')
+    if da.shape != kept.kept.shape:
+        raise ValueError('da must be shaped like the forward call\'s z, %s, got %s' % (tuple(kept.kept.shape), tuple(da.shape)))
+    dr, rows, c, ldd = _rows(da, 'da')
+    qr, _, _, ldk = _codes(kept.kept, dev, 'the checkpoint')
+    dz = torch.empty(da.shape, dtype=da.dtype, device=dev)
+    grads = torch.empty((2, c), dtype=torch.float32, device=dev)
+    ws, nbytes, keep = _scratch(lib.yh_norm_act_workspace_bytes, dev, rows, c, kind)
+    _call(dev, lib.yh_norm_act_backward, dr.data_ptr(), ldd, kind, rows, c, qr.data_ptr(), ldk, kept.scale.data_ptr(),
+          kept.gamma.data_ptr(), kept.invstd.data_ptr(), kept.slope, dz.data_ptr(), c,
+          grads.data_ptr(), grads.data_ptr() + 4 * c, ws, nbytes)
+    return dz, grads[0], grads[1]
