@@ -23,6 +23,18 @@ Reference behaviour kept on purpose:
   * the second header of YOLOv3 is built with 256 filters (YOLOv3.py:86).
 Checkpoints are torch state_dicts: TensorFlow checkpoints cannot be read
 without TensorFlow.
+
+Two options of both stacks have no counterpart in the reference (quant.py; they
+need a HIP device, and are float32 training on MIOpen without them):
+  * pointwise='int8': the 1x1 convolutions are products of 8-bit integers with a
+    scale for each pixel and each output channel, in training (straight-through
+    gradients) and in inference;
+  * checkpoints='int8': what a layer keeps for the backward pass is kept in 8 bits:
+    the convolution's input as row codes (a byte a value), the normalisation and
+    activation as one byte a value (the activation's side exactly, the normalised
+    value in seven bits).  The forward pass is computed as before, the
+    normalisation by the library's own kernels.  Three float32 tensors a layer
+    (12 bytes a value) become two bytes.
 """
 import math
 import os
@@ -32,6 +44,8 @@ import torch
 import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
+
+from . import quant
 
 IMAGE_MEAN = (123.68, 116.779, 103.979)        # YOLOv3.py:66 / YOLOv2.py:60
 BN_EPSILON = 1e-3
@@ -65,7 +79,10 @@ def _variance_scaling_(weight):
 class ConvBN(nn.Module):
     """conv2d('same', bias) -> batch normalisation -> optional leaky ReLU(0.1):
     _conv_layer of YOLOv3.py:496-509; YOLOv2.py:355-366 without the activation,
-    which YOLOv2 applies at the call site."""
+    which YOLOv2 applies at the call site.  forward's `residual` is added to the
+    result (the shortcut of a residual unit)."""
+
+    pointwise = checkpoints = 'float32'        # or 'int8': _Provider sets them
 
     def __init__(self, cin, cout, kernel, stride=1, activation=True, init='variance_scaling'):
         super().__init__()
@@ -78,9 +95,25 @@ class ConvBN(nn.Module):
             nn.init.xavier_uniform_(self.conv.weight)
         nn.init.zeros_(self.conv.bias)
 
-    def forward(self, x):
-        x = self.bn(self.conv(_pad_same(x, self.kernel, self.stride)))
-        return F.leaky_relu(x, LEAKY_SLOPE) if self.activation else x
+    def forward(self, x, residual=None):
+        x = _pad_same(x, self.kernel, self.stride)
+        if self.pointwise == 'int8' and self.kernel == 1 and self.stride == 1:
+            weight = self.conv.weight.reshape(self.conv.out_channels, -1)
+            x = quant.linear_int8(x.permute(0, 2, 3, 1), weight, self.conv.bias).permute(0, 3, 1, 2)
+        elif self.checkpoints == 'int8':
+            x = quant.conv_kept(x, self.conv.weight, self.conv.bias, self.stride)
+        else:
+            x = self.conv(x)
+        if self.checkpoints == 'int8' and self.bn.training:
+            self.bn.num_batches_tracked.add_(1)
+            return quant.norm_act_kept(x.permute(0, 2, 3, 1), self.bn.weight, self.bn.bias, self.bn.eps,
+                                       LEAKY_SLOPE if self.activation else 1.0,
+                                       None if residual is None else residual.permute(0, 2, 3, 1),
+                                       (self.bn.running_mean, self.bn.running_var), self.bn.momentum).permute(0, 3, 1, 2)
+        x = self.bn(x)
+        if self.activation:
+            x = F.leaky_relu(x, LEAKY_SLOPE)
+        return x if residual is None else residual + x
 
 
 class DarknetBlock(nn.Module):
@@ -96,7 +129,10 @@ class DarknetBlock(nn.Module):
     def forward(self, x):
         x = self.down(x)
         for unit in self.units:
-            x = x + unit(x)
+            if unit[1].checkpoints == 'int8':
+                x = unit[1](unit[0](x), residual=x)          # the shortcut inside the normalisation's kernel
+            else:
+                x = x + unit(x)
         return x
 
 
@@ -134,9 +170,13 @@ class Yolo3Header(nn.Module):
 class _Provider(nn.Module):
     """What the two stacks share: image intake, optimiser, checkpoints."""
 
-    def __init__(self, data_format, weight_decay, momentum):
+    def __init__(self, data_format, weight_decay, momentum, pointwise='float32', checkpoints='float32'):
         super().__init__()
         assert data_format in ('channels_first', 'channels_last')
+        for name, value in (('pointwise', pointwise), ('checkpoints', checkpoints)):
+            if value not in ('float32', 'int8'):
+                raise ValueError("%s must be 'float32' or 'int8', got %r" % (name, value))
+        self.pointwise, self.checkpoints = pointwise, checkpoints
         self.data_format = data_format
         self.weight_decay = float(weight_decay)
         self.momentum = float(momentum)
@@ -144,6 +184,9 @@ class _Provider(nn.Module):
         self._velocity = None
 
     def _finish_init(self):
+        for layer in self.modules():
+            if isinstance(layer, ConvBN):
+                layer.pointwise, layer.checkpoints = self.pointwise, self.checkpoints
         self.to(memory_format=torch.channels_last)
         self.train()                        # batch statistics always, as in the reference's graph
 
@@ -216,8 +259,9 @@ class Darknet53Heads(_Provider):
     """images -> [pred1 (stride 32), pred2 (16), pred3 (8)], each
     [B, H, W, num_priors * (num_classes + 5)] (YOLOv3.py:81-91)."""
 
-    def __init__(self, num_classes, num_priors, data_format='channels_last', weight_decay=0.0, momentum=0.9):
-        super().__init__(data_format, weight_decay, momentum)
+    def __init__(self, num_classes, num_priors, data_format='channels_last', weight_decay=0.0, momentum=0.9,
+                 pointwise='float32', checkpoints='float32'):
+        super().__init__(data_format, weight_decay, momentum, pointwise, checkpoints)
         final_units = (num_classes + 5) * num_priors
         # scope 'backone' (sic, YOLOv3.py:82): _feature_extractor, YOLOv3.py:387-394
         self.backone = nn.ModuleDict(dict(
@@ -255,8 +299,9 @@ class Darknet19Head(_Provider):
                 (1024, 3), (512, 1), (1024, 3), (512, 1), (1024, 3)]
     HEAD = [(1024, 3), (512, 1), (1024, 3), (512, 1), (1024, 3)]
 
-    def __init__(self, num_classes, num_priors, data_format='channels_last', weight_decay=0.0, momentum=0.9):
-        super().__init__(data_format, weight_decay, momentum)
+    def __init__(self, num_classes, num_priors, data_format='channels_last', weight_decay=0.0, momentum=0.9,
+                 pointwise='float32', checkpoints='float32'):
+        super().__init__(data_format, weight_decay, momentum, pointwise, checkpoints)
         final_units = (num_classes + 5) * num_priors
         layers, cin = [], 3
         for spec in self.FEATURES:

@@ -262,3 +262,99 @@ def norm_act_backward(da, kept):
           kept.gamma.data_ptr(), kept.invstd.data_ptr(), kept.slope, dz.data_ptr(), c,
           grads.data_ptr(), grads.data_ptr() + 4 * c, ws, nbytes)
     return dz, grads[0], grads[1]
+
+
+# ------------------------------------------------------------------ autograd
+class _LinearInt8(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, keep):
+        w_codes, w_scale = quantize_rows(weight)
+        if not keep:
+            return matmul_int8(x, w_codes, w_scale, bias)
+        y, codes, scale = matmul_int8(x, w_codes, w_scale, bias, want_codes=True)
+        ctx.save_for_backward(codes, scale, w_codes, w_scale)
+        ctx.types = weight.dtype, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        codes, scale, w_codes, w_scale = ctx.saved_tensors
+        dx = input_grad(dy, w_codes, w_scale) if ctx.needs_input_grad[0] else None
+        dw = db = None
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dw, db = weight_grad(dy, codes, scale, want_bias=True)
+            dw = dw.to(ctx.types[0])
+            db = None if ctx.types[1] is None else db.to(ctx.types[1])
+        return dx, dw, db, None
+
+
+def linear_int8(x, weight, bias=None):
+    """x [..., K] times weight [N, K] (float, quantised by its rows in the call) plus bias, in 8-bit integers, with
+    gradients: the codes of x are the checkpoint that the weights' gradient is computed from."""
+    return _LinearInt8.apply(x, weight, bias, torch.is_grad_enabled())
+
+
+KEEP_CODES_FROM = 8          # channels; shorter rows take no less memory as codes (rows of 16 bytes and a scale)
+
+
+class _ConvKept(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, stride):
+        y = F.conv2d(x, weight, bias, stride)
+        codes, scale = quantize_rows(x.permute(0, 2, 3, 1))
+        ctx.save_for_backward(codes, scale, weight)
+        ctx.stride, ctx.has_bias, ctx.dtype = stride, bias is not None, x.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        codes, scale, weight = ctx.saved_tensors
+        n, k = weight.shape[:2]
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if weight.shape[2:] == (1, 1) and ctx.stride == 1:
+            rows = dy.permute(0, 2, 3, 1)
+            dx = dw = db = None
+            if need_x:
+                dx = (rows.reshape(-1, n) @ weight.reshape(n, k)).view(codes.shape).permute(0, 3, 1, 2)
+            if need_w or need_b:
+                dw, db = weight_grad(rows, codes, scale, want_bias=True)
+                dw, db = dw.to(weight.dtype).view(weight.shape), db.to(weight.dtype)
+            return dx, dw, db if ctx.has_bias else None, None
+        x = dequantize_rows(codes, scale, ctx.dtype).permute(0, 3, 1, 2)
+        s = [ctx.stride, ctx.stride]
+        dx, dw, db = torch.ops.aten.convolution_backward(dy.contiguous(memory_format=torch.channels_last), x, weight, [n] if ctx.has_bias else None,
+                                                         s, [0, 0], [1, 1], False, [0, 0], 1, [need_x, need_w, need_b and ctx.has_bias])
+        return dx, dw, db, None
+
+
+def conv_kept(x, weight, bias, stride):
+    """F.conv2d(x, weight, bias, stride) of an NCHW tensor that keeps x for the backward pass as row codes (a byte a
+    value and a scale a pixel) in the place of x itself.  The output is the plain convolution's; the weights'
+    gradient is that of the values the codes stand for."""
+    if not torch.is_grad_enabled() or x.shape[1] < KEEP_CODES_FROM:
+        return F.conv2d(x, weight, bias, stride)
+    return _ConvKept.apply(x, weight, bias, int(stride))
+
+
+class _NormAct(Function):
+    @staticmethod
+    def forward(ctx, z, gamma, beta, eps, slope, residual, running, momentum, keep):
+        a, kept = norm_act(z, gamma, beta, eps, slope, residual, running, momentum, want_kept=keep)
+        if keep:
+            ctx.save_for_backward(kept.kept, kept.scale, kept.mean, kept.invstd, gamma)
+            ctx.slope = kept.slope
+        return a
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, da):
+        kept, scale, mean, invstd, gamma = ctx.saved_tensors
+        dz, dgamma, dbeta = norm_act_backward(da, NormKept(kept, scale, mean, invstd, gamma.detach(), ctx.slope))
+        return dz, dgamma, dbeta, None, None, da if ctx.needs_input_grad[5] else None, None, None, None
+
+
+def norm_act_kept(z, gamma, beta, eps, slope, residual=None, running=None, momentum=0.01):
+    """norm_act with gradients for z, gamma, beta and the residual, from its 8-bit checkpoint."""
+    return _NormAct.apply(z, gamma, beta, eps, slope, residual, running, momentum, torch.is_grad_enabled())

@@ -91,7 +91,9 @@ class YOLOv2:
         """_build_graph's convolution stack (YOLOv2.py:75-93): built on first use, when
         images rather than a head tensor arrive and no provider was configured."""
         from .backbone import Darknet19Head
-        net = Darknet19Head(self.num_classes, self.num_priors, self.data_format, self.weight_decay)
+        net = Darknet19Head(self.num_classes, self.num_priors, self.data_format, self.weight_decay,
+                            pointwise=self.config.get('pointwise', 'float32'),
+                            checkpoints=self.config.get('checkpoints', 'float32'))
         return net.to(torch.device('cuda', torch.cuda.current_device()))
 
     def _is_image_batch(self, x):

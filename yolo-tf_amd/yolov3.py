@@ -13,6 +13,8 @@ built and used:
     (or NCHW when data_format == 'channels_first', transposed here exactly as
     YOLOv3.py:88-91 does).  Without a provider `images` must already be that
     list of head tensors.
+  * config['pointwise'], config['checkpoints'] (optional, 'float32' or 'int8'): the
+    8-bit options of the stack built here (backbone.py).
   * data_provider['train_generator'] = (initializer, iterator): `initializer`
     is a callable (or None) run at the start of an epoch, `iterator` yields
     (images_or_heads, ground_truth[B, pad, 5]) batches; they stand where the
@@ -117,7 +119,9 @@ class YOLOv3:
         """_build_graph's convolution stack (YOLOv3.py:81-91): built on first use, when
         images rather than head tensors arrive and no provider was configured."""
         from .backbone import Darknet53Heads
-        net = Darknet53Heads(self.num_classes, self.num_priors, self.data_format, self.weight_decay)
+        net = Darknet53Heads(self.num_classes, self.num_priors, self.data_format, self.weight_decay,
+                             pointwise=self.config.get('pointwise', 'float32'),
+                             checkpoints=self.config.get('checkpoints', 'float32'))
         return net.to(torch.device('cuda', torch.cuda.current_device()))
 
     def _heads_from(self, images):
