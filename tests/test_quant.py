@@ -23,7 +23,7 @@ def test_no_cpu_path():
     g = torch.ones(8)
     for call in (lambda: quant.quantize_rows(x), lambda: quant.dequantize_rows(q, s), lambda: quant.matmul_int8(x, q, s),
                  lambda: quant.weight_grad(x, q, s), lambda: quant.input_grad(x, q, s), lambda: quant.norm_act(x, g, g, 1e-3, 0.1),
-                 lambda: quant.norm_act_backward(x, quant.NormKept(q, s, g, g, g, 0.1))):
+                 lambda: quant.norm_act_backward(x, quant.NormKept(q, (3, 8), 3, 16, g, 0.1))):
         with pytest.raises(RuntimeError, match='no CPU path'):
             call()
     with pytest.raises(TypeError, match='torch tensor'):

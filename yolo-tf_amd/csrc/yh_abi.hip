@@ -460,7 +460,14 @@ int report(int code, const char *fmt, ...)
     return code;
 }
 int report_hip(hipError_t e, const char *what) { return hip_fail(e, what); }
-int require_device() { return ensure_device(); }
+int require_device()
+{
+    static std::atomic<bool> found{false};               // a device once seen stays
+    if (found.load(std::memory_order_relaxed)) return YH_OK;
+    const int rc = ensure_device();
+    if (rc == YH_OK) found.store(true, std::memory_order_relaxed);
+    return rc;
+}
 }  // namespace yh
 
 extern "C" {

@@ -338,23 +338,35 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
 template <class T, int BA, int BB>
 __global__ __launch_bounds__(kThreads, 2) void k_weight_grad(const T *dy, int64_t ldd, const int8_t *codes, int64_t ldc, const float *scale,
                                                              int64_t rows, int n, int k, int64_t rows_per_piece, int tiles_k, int tiles,
-                                                             float *dw, float *db)
+                                                             float *dw, float *db, int64_t pitch)
 {
     const int64_t id = xcd_run(blockIdx.x, gridDim.x);
     const int64_t piece = id / tiles;
     const int tile = (int)(id % tiles), a0 = tile / tiles_k * BA, b0 = tile % tiles_k * BB;
     const int64_t r0 = piece * rows_per_piece, r1 = min(rows, r0 + rows_per_piece);
     split_tile<T, true, BA, BB, float, true>(dy, ldd, scale, codes, ldc, a0, n, b0, k, r0, r1,
-                                             dw + piece * n * k, k, db && b0 == 0 ? db + piece * n : nullptr);
+                                             dw + piece * pitch, k, db && b0 == 0 ? db + piece * pitch : nullptr);
 }
 
-__global__ __launch_bounds__(kThreads) void k_add_pieces(const float *part, int pieces, int64_t count, float *out)
+// out[i] = sum of part[p][i] over the pieces, in 64 bits; the first `cut` values are dw, the others db.  A workgroup takes
+// `wide` values; its 256 / wide groups of threads add pieces in turn, and their sums are added in order.
+__global__ __launch_bounds__(kThreads) void k_add_pieces(const float *part, int pieces, int64_t count, int64_t cut, int wide, float *dw, float *db)
 {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= count) return;
+    __shared__ double buf[kThreads];
+    const int col = threadIdx.x & (wide - 1), group = threadIdx.x / wide, groups = kThreads / wide;
+    const int64_t i = (int64_t)blockIdx.x * wide + col;
     double s = 0.0;
-    for (int p = 0; p < pieces; ++p) s += (double)part[p * count + i];
-    out[i] = (float)s;
+    if (i < count) {
+#pragma unroll 8
+        for (int p = group; p < pieces; p += groups) s += (double)part[p * count + i];
+    }
+    buf[threadIdx.x] = s;
+    __syncthreads();
+    if (group == 0 && i < count) {
+        for (int g = 1; g < groups; ++g) s += buf[g * wide + col];
+        if (i < cut) dw[i] = (float)s;
+        else db[i - cut] = (float)s;
+    }
 }
 
 __global__ __launch_bounds__(kThreads) void k_fill_zero(float *p, int64_t count)
@@ -433,11 +445,12 @@ hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, 
     }
     const GradPlan p = plan_weight_grad(rows, n, k);
     float *pw = p.pieces > 1 ? static_cast<float *>(workspace) : dw;
-    float *pb = !db ? nullptr : p.pieces > 1 ? pw + p.pieces * count : db;
+    float *pb = !db ? nullptr : p.pieces > 1 ? pw + count : db;
+    const int64_t pitch = db ? count + n : count;              // a piece: dw, then db
     with_type(dy.type, [&](auto t) {
         using T = decltype(t);
 #define CALL(BA, BB) k_weight_grad<T, BA, BB><<<dim3((unsigned)(p.tiles * p.pieces)), kThreads, 0, st>>>(                   \
-            static_cast<const T *>(dy.p), dy.ld, codes, ldc, scale, rows, n, k, p.rows_per_piece, p.tiles_k, p.tiles, pw, pb)
+            static_cast<const T *>(dy.p), dy.ld, codes, ldc, scale, rows, n, k, p.rows_per_piece, p.tiles_k, p.tiles, pw, pb, pitch)
         if (p.ba == 64 && p.bb == 64) CALL(64, 64);
         else if (p.ba == 64) CALL(64, 128);
         else if (p.bb == 64) CALL(128, 64);
@@ -445,8 +458,10 @@ hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, 
 #undef CALL
     });
     if (p.pieces > 1) {
-        k_add_pieces<<<dim3(blocks_for(count)), kThreads, 0, st>>>(pw, p.pieces, count, dw);
-        if (db) k_add_pieces<<<dim3(blocks_for(n)), kThreads, 0, st>>>(pb, p.pieces, n, db);
+        // few pieces: a thread a value; many: eight pieces a thread, down to 16 neighbouring values (64 bytes) a workgroup
+        int wide = kThreads;
+        while (wide > 16 && p.pieces * wide > 8 * kThreads) wide /= 2;
+        k_add_pieces<<<dim3((unsigned)((pitch + wide - 1) / wide)), kThreads, 0, st>>>(pw, p.pieces, pitch, count, wide, dw, db);
     }
     return hipGetLastError();
 }

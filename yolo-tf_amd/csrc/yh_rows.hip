@@ -151,28 +151,36 @@ __global__ __launch_bounds__(kThreads) void k_dequantize(const int8_t *codes, in
 // workgroup and channel, a small launch that adds the partials in a fixed order, and an elementwise pass.
 
 // A workgroup's threads over (channel vectors, rows) in the reductions.
-struct ReducePlan { int tx, ty, slabs, blocks; int64_t rows_per_block; };
+struct ReducePlan { int tx, ty, slabs, blocks; };
 ReducePlan plan_reduce(int64_t rows, int cols, int V)
 {
     const int cv = (cols + V - 1) / V;
     ReducePlan p;
-    p.tx = std::min(64, pow2_at_least(cv));
+    // Up to 1024 rows one workgroup takes all rows of a slab of four vectors (64 bytes a row) and finishes by itself:
+    // the launch that adds the partials costs more than what the spread over workgroups wins (13 x 13 x 1024 bf16, both
+    // passes of a step: 22 us of kernels with it).
+    const bool alone = rows <= 1024;
+    p.tx = std::min(alone ? 4 : 64, pow2_at_least(cv));
     p.ty = kThreads / p.tx;
     p.slabs = (cv + p.tx - 1) / p.tx;
+    if (alone) {
+        p.blocks = 1;
+        return p;
+    }
     // about 1024 workgroups in all (four a compute unit), each thread with at least eight rows
     const int64_t by_rows = (rows + p.ty * 8 - 1) / ((int64_t)p.ty * 8);
     const int64_t want = std::max(1, 1024 / p.slabs);
-    const int64_t blocks = std::max<int64_t>(1, std::min(want, by_rows));
-    p.rows_per_block = (rows + blocks - 1) / blocks;
-    p.blocks = (int)((rows + p.rows_per_block - 1) / p.rows_per_block);
+    p.blocks = (int)std::max<int64_t>(1, std::min(want, by_rows));
     return p;
 }
 
-// Adds the threads' pairs over ty and writes the workgroup's pair of each channel: part[2][cols][blocks].
+// Adds the threads' pairs over ty, into those with ty == 0, and writes the workgroup's pair of each channel to
+// part[2][cols][blocks] where there is more than one workgroup.
 template <int V>
 __device__ __forceinline__ void reduce_pairs(double (&s1)[V], double (&s2)[V], int tx, int ty, int TX, int cvec, int cols, double *part, int blocks)
 {
     __shared__ double buf[kThreads * V];
+#pragma unroll
     for (int which = 0; which < 2; ++which) {
         double (&s)[V] = which ? s2 : s1;
         __syncthreads();
@@ -188,69 +196,126 @@ __device__ __forceinline__ void reduce_pairs(double (&s1)[V], double (&s2)[V], i
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const int c = cvec * V + j;
-                if (c < cols) part[((int64_t)which * cols + c) * blocks + blockIdx.x] = buf[j * kThreads + tx];
+                s[j] = buf[j * kThreads + tx];
+                if (blocks > 1 && c < cols) part[((int64_t)which * cols + c) * blocks + blockIdx.x] = s[j];
             }
     }
 }
 
+// What follows from a channel's sums of (z - first) and of its square.
+struct NormStats {
+    int64_t rows;
+    double eps, momentum;
+    float *mean, *invstd, *running_mean, *running_var;
+    __device__ __forceinline__ void finish(int c, float first, double s1, double s2) const
+    {
+        const double m = (double)rows, d = s1 / m, mu = (double)first + d;
+        double var = s2 / m - d * d;
+        if (var < 0.0) var = 0.0;                        // a NaN stays one
+        mean[c] = (float)mu;
+        invstd[c] = (float)(1.0 / sqrt(var + eps));
+        if (running_mean) {
+            running_mean[c] = (float)((1.0 - momentum) * (double)running_mean[c] + momentum * mu);
+            running_var[c] = (float)((1.0 - momentum) * (double)running_var[c] + momentum * (rows > 1 ? var * (m / (m - 1.0)) : var));
+        }
+    }
+};
+
+// What the elementwise pass of the backward takes from a channel's sums: coef = gamma * invstd, dbeta / M, dgamma / M.
+struct NormGrads {
+    int64_t rows;
+    int cols;
+    const float *gamma, *invstd;
+    float *dgamma, *dbeta, *coef;
+    __device__ __forceinline__ void finish(int c, double b, double g) const
+    {
+        dbeta[c] = (float)b;
+        dgamma[c] = (float)g;
+        coef[c] = gamma[c] * invstd[c];
+        coef[cols + c] = (float)(b / (double)rows);
+        coef[2 * (int64_t)cols + c] = (float)(g / (double)rows);
+    }
+};
+
 template <class T>
-__global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int TX, int64_t rows_per_block, double *part)
+__global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int TX, double *part,
+                                                         NormStats out)
 {
     constexpr int V = RowVec<T>::V, U = 4;
     const int tx = threadIdx.x & (TX - 1), ty = threadIdx.x / TX, TY = kThreads / TX;
     const int cvec = blockIdx.y * TX + tx, c = cvec * V, left = cols - c;
-    const int64_t r0 = (int64_t)blockIdx.x * rows_per_block, r1 = min(rows, r0 + rows_per_block);
     double s1[V], s2[V];
     float first[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
     load_vec<T, V>(first, z + c, left);
     const T *p = z + c;
-    for (int64_t r = r0 + ty; r < r1; r += (int64_t)U * TY) {
-        float v[U][V];
+    const int64_t step = (int64_t)gridDim.x * U * TY;
+    const auto add = [&](const float (&v)[V]) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) load_vec<T, V>(v[i], p + (r + i * TY) * ldz, r + i * TY < r1 ? left : 0);
+        for (int j = 0; j < V; ++j) {
+            const double d = (double)v[j] - (double)first[j];
+            s1[j] += d;
+            s2[j] = __builtin_fma(d, d, s2[j]);
+        }
+    };
+    int64_t r = (int64_t)blockIdx.x * U * TY + ty;
+    if (left >= V)                                   // whole vectors, whole groups of rows: nothing to ask in the loop
+        for (; r + (U - 1) * TY < rows; r += step) {
+            float v[U][V];
 #pragma unroll
-        for (int i = 0; i < U; ++i)
-            if (r + i * TY < r1)
+            for (int i = 0; i < U; ++i) load_vec<T, V>(v[i], p + (r + i * TY) * ldz, V);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const double d = (double)v[i][j] - (double)first[j];
-                    s1[j] += d;
-                    s2[j] = __builtin_fma(d, d, s2[j]);
-                }
-    }
+            for (int i = 0; i < U; ++i) add(v[i]);
+        }
+    for (; r < rows; r += step)
+        for (int i = 0; i < U && r + i * TY < rows; ++i) {
+            float v[V];
+            load_vec<T, V>(v, p + (r + i * TY) * ldz, left);
+            add(v);
+        }
     reduce_pairs<V>(s1, s2, tx, ty, TX, cvec, cols, part, gridDim.x);
+    if (gridDim.x == 1 && ty == 0)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < left) out.finish(c + j, first[j], s1[j], s2[j]);
 }
 
-// One wavefront a channel: the partials in a fixed order, whatever ran first.
-__device__ __forceinline__ double sum_partials(const double *p, int blocks, int lane)
+// A channel's pair of sums over its partials, by `lanes` threads (64: a wavefront, or 256: the workgroup; few partials
+// take the wavefront) in a fixed order, whatever ran first.  Whole in the thread with at == 0.
+__device__ __forceinline__ void sum_partials(const double *p, const double *q, int blocks, int at, int lanes, double &s1, double &s2)
 {
-    double s = 0.0;
-    for (int i = lane; i < blocks; i += 64) s += p[i];
-    for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
-    return s;
+    __shared__ double buf[2][kThreads / 64];
+    s1 = s2 = 0.0;
+#pragma unroll 4
+    for (int i = at; i < blocks; i += lanes) {
+        s1 += p[i];
+        s2 += q[i];
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+        s1 += __shfl_xor(s1, o);
+        s2 += __shfl_xor(s2, o);
+    }
+    if (lanes == 64) return;
+    if ((at & 63) == 0) {
+        buf[0][at >> 6] = s1;
+        buf[1][at >> 6] = s2;
+    }
+    __syncthreads();
+    if (at == 0)
+        for (int i = 1; i < kThreads / 64; ++i) {
+            s1 += buf[0][i];
+            s2 += buf[1][i];
+        }
 }
 
 template <class T>
-__global__ __launch_bounds__(kThreads) void k_norm_stats_finish(const double *part, int blocks, const T *z, int64_t rows, int cols, double eps,
-                                                                float *mean, float *invstd, float *running_mean, float *running_var, double momentum)
+__global__ __launch_bounds__(kThreads) void k_norm_stats_finish(const double *part, int blocks, const T *z, int cols, int lanes, NormStats out)
 {
-    const int c = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (c >= cols) return;
-    const double m = (double)rows;
-    const double d = sum_partials(part + (int64_t)c * blocks, blocks, lane) / m;
-    const double e = sum_partials(part + ((int64_t)cols + c) * blocks, blocks, lane) / m;
-    if (lane) return;
-    const double mu = (double)(float)z[c] + d;
-    double var = e - d * d;
-    if (var < 0.0) var = 0.0;                        // a NaN stays one
-    mean[c] = (float)mu;
-    invstd[c] = (float)(1.0 / sqrt(var + eps));
-    if (running_mean) {
-        running_mean[c] = (float)((1.0 - momentum) * (double)running_mean[c] + momentum * mu);
-        running_var[c] = (float)((1.0 - momentum) * (double)running_var[c] + momentum * (rows > 1 ? var * (m / (m - 1.0)) : var));
-    }
+    const int per = kThreads / lanes, c = min((int)blockIdx.x * per + (int)threadIdx.x / lanes, cols - 1), at = threadIdx.x & (lanes - 1);
+    double s1, s2;
+    sum_partials(part + (int64_t)c * blocks, part + ((int64_t)cols + c) * blocks, blocks, at, lanes, s1, s2);
+    if (at == 0 && (int)blockIdx.x * per + (int)threadIdx.x / lanes < cols) out.finish(c, (float)z[c], s1, s2);
 }
 
 template <class T, int IT>
@@ -371,52 +436,62 @@ __device__ __forceinline__ bool kept_side(uint32_t w, int i) { return (w >> (8 *
 
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
-                                                             int64_t rows, int cols, float slope, int TX, int64_t rows_per_block, double *part)
+                                                             int64_t rows, int cols, float slope, int TX, double *part,
+                                                             NormGrads out)
 {
     constexpr int V = RowVec<T>::V, U = 4;
     const int tx = threadIdx.x & (TX - 1), ty = threadIdx.x / TX, TY = kThreads / TX;
     const int cvec = blockIdx.y * TX + tx, c = cvec * V, left = cols - c;
-    const int64_t r0 = (int64_t)blockIdx.x * rows_per_block, r1 = min(rows, r0 + rows_per_block);
     double s1[V], s2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
-    for (int64_t r = r0 + ty; r < r1; r += (int64_t)U * TY) {
-        float v[U][V], s[U];
-        uint32_t w[U][V / 4];
+    const int64_t step = (int64_t)gridDim.x * U * TY;
+    const auto add = [&](const float (&v)[V], const uint32_t (&w)[V / 4], float s) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int64_t rr = r + i * TY;
-            const int l = rr < r1 ? left : 0;
-            load_vec<T, V>(v[i], da + rr * ldd + c, l);
-            load_bytes<V>(w[i], kept + rr * ldk + c, l);
-            s[i] = rr < r1 ? scale[rr] : 0.0f;
+        for (int j = 0; j < V; ++j) {
+            const float du = kept_side(w[j / 4], j % 4) ? v[j] : slope * v[j];
+            const float xq = kept_code(w[j / 4], j % 4) * s;
+            s1[j] += (double)du;
+            s2[j] = __builtin_fma((double)du, (double)xq, s2[j]);
         }
+    };
+    int64_t r = (int64_t)blockIdx.x * U * TY + ty;
+    if (left >= V)
+        for (; r + (U - 1) * TY < rows; r += step) {
+            float v[U][V], s[U];
+            uint32_t w[U][V / 4];
 #pragma unroll
-        for (int i = 0; i < U; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float du = kept_side(w[i][j / 4], j % 4) ? v[i][j] : slope * v[i][j];
-                const float xq = kept_code(w[i][j / 4], j % 4) * s[i];
-                s1[j] += (double)du;
-                s2[j] = __builtin_fma((double)du, (double)xq, s2[j]);
+            for (int i = 0; i < U; ++i) {
+                const int64_t rr = r + i * TY;
+                load_vec<T, V>(v[i], da + rr * ldd + c, V);
+                load_bytes<V>(w[i], kept + rr * ldk + c, V);
+                s[i] = scale[rr];
             }
-    }
+#pragma unroll
+            for (int i = 0; i < U; ++i) add(v[i], w[i], s[i]);
+        }
+    for (; r < rows; r += step)
+        for (int i = 0; i < U && r + i * TY < rows; ++i) {
+            const int64_t rr = r + i * TY;
+            float v[V];
+            uint32_t w[V / 4];
+            load_vec<T, V>(v, da + rr * ldd + c, left);
+            load_bytes<V>(w, kept + rr * ldk + c, left);
+            add(v, w, scale[rr]);
+        }
     reduce_pairs<V>(s1, s2, tx, ty, TX, cvec, cols, part, gridDim.x);
+    if (gridDim.x == 1 && ty == 0)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < left) out.finish(c + j, s1[j], s2[j]);
 }
 
-__global__ __launch_bounds__(kThreads) void k_norm_grad_finish(const double *part, int blocks, int64_t rows, int cols, const float *gamma, const float *invstd,
-                                                               float *dgamma, float *dbeta, float *coef)
+__global__ __launch_bounds__(kThreads) void k_norm_grad_finish(const double *part, int blocks, int cols, int lanes, NormGrads out)
 {
-    const int c = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (c >= cols) return;
-    const double b = sum_partials(part + (int64_t)c * blocks, blocks, lane);
-    const double g = sum_partials(part + ((int64_t)cols + c) * blocks, blocks, lane);
-    if (lane) return;
-    dbeta[c] = (float)b;
-    dgamma[c] = (float)g;
-    coef[c] = gamma[c] * invstd[c];
-    coef[cols + c] = (float)(b / (double)rows);
-    coef[2 * (int64_t)cols + c] = (float)(g / (double)rows);
+    const int per = kThreads / lanes, c = min((int)blockIdx.x * per + (int)threadIdx.x / lanes, cols - 1), at = threadIdx.x & (lanes - 1);
+    double b, g;
+    sum_partials(part + (int64_t)c * blocks, part + ((int64_t)cols + c) * blocks, blocks, at, lanes, b, g);
+    if (at == 0 && (int)blockIdx.x * per + (int)threadIdx.x / lanes < cols) out.finish(c, b, g);
 }
 
 template <class T, int IT>
@@ -530,8 +605,11 @@ hipError_t launch_norm_forward(const Rows &z, const Rows &res, int64_t rows, int
         using T = decltype(t);
         const T *p = static_cast<const T *>(z.p), *q = static_cast<const T *>(res.p);
         const ReducePlan d = plan_reduce(rows, cols, RowVec<T>::V);
-        k_norm_stats<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, rows, cols, z.ld, d.tx, d.rows_per_block, part);
-        k_norm_stats_finish<T><<<dim3(waves_to_blocks(cols)), kThreads, 0, st>>>(part, d.blocks, p, rows, cols, eps, mean, invstd, running_mean, running_var, momentum);
+        const NormStats out{rows, eps, momentum, mean, invstd, running_mean, running_var};
+        k_norm_stats<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, rows, cols, z.ld, d.tx, part, out);
+        const int lanes = d.blocks > 64 ? kThreads : 64;
+        if (d.blocks > 1)
+            k_norm_stats_finish<T><<<dim3((cols * lanes + kThreads - 1) / kThreads), kThreads, 0, st>>>(part, d.blocks, p, cols, lanes, out);
         const RowPlan r = plan_row(cols, RowVec<T>::V);
         if (r.vecs > 6) {
             k_norm_apply_long<T><<<dim3(row_blocks(rows)), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope,
@@ -557,8 +635,11 @@ hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, cons
         const T *p = static_cast<const T *>(da.p);
         const ReducePlan d = plan_reduce(rows, cols, RowVec<T>::V);
         float *coef = reinterpret_cast<float *>(part + 2 * (int64_t)cols * d.blocks);
-        k_norm_grad_sums<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, da.ld, kept, ldk, scale, rows, cols, slope, d.tx, d.rows_per_block, part);
-        k_norm_grad_finish<<<dim3(waves_to_blocks(cols)), kThreads, 0, st>>>(part, d.blocks, rows, cols, gamma, invstd, dgamma, dbeta, coef);
+        const NormGrads out{rows, cols, gamma, invstd, dgamma, dbeta, coef};
+        k_norm_grad_sums<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, da.ld, kept, ldk, scale, rows, cols, slope, d.tx, part, out);
+        const int lanes = d.blocks > 64 ? kThreads : 64;
+        if (d.blocks > 1)
+            k_norm_grad_finish<<<dim3((cols * lanes + kThreads - 1) / kThreads), kThreads, 0, st>>>(part, d.blocks, cols, lanes, out);
         const RowPlan r = plan_row(cols, RowVec<T>::V);
         const int vecs = std::min(4, r.vecs), step = (vecs <= 1 ? 1 : vecs <= 2 ? 2 : 4) * r.lanes * RowVec<T>::V;
         const unsigned blocks = std::min(2048u, waves_to_blocks((rows * r.lanes + 63) / 64));

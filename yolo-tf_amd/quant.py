@@ -27,31 +27,41 @@ _TYPES = {torch.float32: _abi.YH_FLOAT32, torch.bfloat16: _abi.YH_BFLOAT16, torc
 
 
 # ------------------------------------------------------------------ helpers
+# The smallest calls take a few microseconds on the device, so the host's share counts: no call makes a tensor, a view
+# or a library query that it can do without.
+_sizes = {}                  # workspace sizes by (query, its arguments): they depend on nothing else
+
+
 def _device_of(x, what):
     if not isinstance(x, torch.Tensor):
         raise TypeError('%s must be a torch tensor on a HIP device' % what)
-    if x.device.type != 'cuda':
-        raise RuntimeError('%s must live on a HIP device (got %s); there is no CPU path' % (what, x.device))
-    return x.device
+    dev = x.device
+    if dev.type != 'cuda':
+        raise RuntimeError('%s must live on a HIP device (got %s); there is no CPU path' % (what, dev))
+    return dev
 
 
-def _float_type(x, what):
-    code = _TYPES.get(x.dtype)
+def _float_type(dtype, what):
+    code = _TYPES.get(dtype)
     if code is None:
-        raise ValueError('%s must be float32, bfloat16 or float16, got %s' % (what, x.dtype))
+        raise ValueError('%s must be float32, bfloat16 or float16, got %s' % (what, dtype))
     return code
 
 
 def _rows(x, what):
     """x as [rows, channels] with adjacent channels: (tensor that owns the memory, rows, channels, elements between rows)."""
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError('%s must be [..., channels] with at least one channel, got %s' % (what, tuple(x.shape)))
+    shape = x.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError('%s must be [..., channels] with at least one channel, got %s' % (what, tuple(shape)))
+    cols = shape[-1]
+    if x.is_contiguous():
+        return x, x.numel() // cols, cols, cols
     x = x.detach()
     if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
-    if x.shape[1] > 1 and x.stride(1) != 1:
+        x = x.reshape(-1, cols)
+    if cols > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    rows, cols = x.shape
+    rows = x.shape[0]
     return x, rows, cols, x.stride(0) if rows > 1 else cols
 
 
@@ -59,8 +69,7 @@ def _vector(v, n, dev, what):
     """A float32 vector of n adjacent values on `dev`."""
     if not isinstance(v, torch.Tensor) or v.dtype != torch.float32 or v.device != dev or v.numel() != n:
         raise ValueError('%s must be %d float32 values on %s' % (what, n, dev))
-    v = v.detach()
-    return v if v.is_contiguous() else v.contiguous()
+    return v if v.is_contiguous() else v.detach().contiguous()
 
 
 def _codes(q, dev, what):
@@ -75,27 +84,33 @@ def _new_codes(shape, dev):
     wide = (cols + 15) // 16 * 16
     if wide == cols:
         return torch.empty(shape, dtype=torch.int8, device=dev), cols
-    return torch.empty(tuple(shape[:-1]) + (wide,), dtype=torch.int8, device=dev)[..., :cols], wide
+    return torch.empty(shape[:-1] + (wide,), dtype=torch.int8, device=dev)[..., :cols], wide
 
 
 def _call(dev, fn, *args):
     """One library call on `dev`'s current stream."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
     if torch.cuda.current_device() == dev.index:
-        _abi.check(fn(*args, stream))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
-            _abi.check(fn(*args, stream))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _abi.check(rc)
 
 
-def _scratch(size_fn, dev, *sizes):
+def _scratch(fn_name, dev, *sizes):
     """(pointer, bytes, tensor that keeps it) of a workspace for one call."""
-    n = ctypes.c_size_t(0)
-    _abi.check(size_fn(*sizes, ctypes.byref(n)))
-    if n.value == 0:
+    n = _sizes.get((fn_name, sizes))
+    if n is None:
+        out = ctypes.c_size_t(0)
+        _abi.check(getattr(_abi.load(), fn_name)(*sizes, ctypes.byref(out)))
+        if len(_sizes) > 4096:
+            _sizes.clear()
+        n = _sizes[(fn_name, sizes)] = out.value
+    if n == 0:
         return None, 0, None
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-    return ws.data_ptr(), n.value, ws
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    return ws.data_ptr(), n, ws
 
 
 # ------------------------------------------------------------------ row codes
@@ -103,10 +118,11 @@ def quantize_rows(x):
     """(codes int8 shaped like x, scale float32 [...]) of the rows of x: scale = max|x| / 127, code =
     x / scale rounded.  A row of zeros has the scale 0; one with an infinity or a NaN the scale NaN."""
     dev = _device_of(x, 'x')
-    kind = _float_type(x, 'x')
+    kind = _float_type(x.dtype, 'x')
     xr, rows, cols, ld = _rows(x, 'x')
-    codes, ldc = _new_codes(tuple(x.shape), dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    shape = tuple(x.shape)
+    codes, ldc = _new_codes(shape, dev)
+    scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
     _call(dev, _abi.load().yh_quantize_rows, xr.data_ptr(), kind, ld, rows, cols, codes.data_ptr(), ldc, scale.data_ptr())
     return codes, scale
 
@@ -114,11 +130,11 @@ def quantize_rows(x):
 def dequantize_rows(codes, scale, dtype=torch.float32):
     """The values that row codes stand for: codes * scale, in `dtype`."""
     dev = _device_of(codes, 'codes')
+    kind = _float_type(dtype, 'dtype')
     qr, rows, cols, ld = _codes(codes, dev, 'codes')
     scale = _vector(scale, rows, dev, 'scale')
     x = torch.empty(codes.shape, dtype=dtype, device=dev)
-    _call(dev, _abi.load().yh_dequantize_rows, qr.data_ptr(), ld, scale.data_ptr(), rows, cols, x.data_ptr(),
-          _float_type(x, 'dtype'), cols)
+    _call(dev, _abi.load().yh_dequantize_rows, qr.data_ptr(), ld, scale.data_ptr(), rows, cols, x.data_ptr(), kind, cols)
     return x
 
 
@@ -136,7 +152,8 @@ def matmul_int8(x, w_codes, w_scale, bias=None, x_scale=None, out_dtype=None, wa
     if w_codes.dim() != 2 or wk != k:
         raise ValueError('w_codes must be [N, %d], got %s' % (k, tuple(w_codes.shape)))
     w_scale = _vector(w_scale, n, dev, 'w_scale')
-    bias = None if bias is None else _vector(bias, n, dev, 'bias')
+    if bias is not None:
+        bias = _vector(bias, n, dev, 'bias')
     whole = x.dtype == torch.int8
     if whole:
         if x_scale is None or want_codes:
@@ -146,18 +163,19 @@ def matmul_int8(x, w_codes, w_scale, bias=None, x_scale=None, out_dtype=None, wa
     else:
         if x_scale is not None:
             raise ValueError('x_scale belongs to int8 codes')
-        kind = _float_type(x, 'x')
+        kind = _float_type(x.dtype, 'x')
         out_dtype = x.dtype if out_dtype is None else out_dtype
-    y = torch.empty(tuple(x.shape[:-1]) + (n,), dtype=out_dtype, device=dev)
+    out_kind = _float_type(out_dtype, 'out_dtype')
+    shape = tuple(x.shape)
+    y = torch.empty(shape[:-1] + (n,), dtype=out_dtype, device=dev)
     codes = scale = None
     ldc = 0
     if want_codes:
-        codes, ldc = _new_codes(tuple(x.shape), dev)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    ws, nbytes, keep = _scratch(lib.yh_matmul_int8_workspace_bytes, dev, rows, k, n, kind, 1 if want_codes else 0)
+        codes, ldc = _new_codes(shape, dev)
+        scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    ws, nbytes, keep = _scratch('yh_matmul_int8_workspace_bytes', dev, rows, k, n, kind, 1 if want_codes else 0)
     _call(dev, lib.yh_matmul_int8, xr.data_ptr(), kind, ldx, x_scale.data_ptr() if whole else None, rows, k,
-          wr.data_ptr(), ldw, w_scale.data_ptr(), n, None if bias is None else bias.data_ptr(),
-          y.data_ptr(), _float_type(y, 'out_dtype'), n,
+          wr.data_ptr(), ldw, w_scale.data_ptr(), n, None if bias is None else bias.data_ptr(), y.data_ptr(), out_kind, n,
           codes.data_ptr() if want_codes else None, ldc, scale.data_ptr() if want_codes else None, ws, nbytes)
     return (y, codes, scale) if want_codes else y
 
@@ -166,8 +184,7 @@ def weight_grad(dy, codes, scale, want_bias=False):
     """dw [N, K] float32 = dy^T times the values of the row codes, from dy [..., N] and codes [..., K] with
     scale [...]; with want_bias (dw, db [N]), db the sum of dy's rows."""
     dev = _device_of(dy, 'dy')
-    lib = _abi.load()
-    kind = _float_type(dy, 'dy')
+    kind = _float_type(dy.dtype, 'dy')
     dr, rows, n, ldd = _rows(dy, 'dy')
     qr, qrows, k, ldq = _codes(codes, dev, 'codes')
     if qrows != rows:
@@ -175,8 +192,8 @@ def weight_grad(dy, codes, scale, want_bias=False):
     scale = _vector(scale, rows, dev, 'scale')
     dw = torch.empty((n, k), dtype=torch.float32, device=dev)
     db = torch.empty((n,), dtype=torch.float32, device=dev) if want_bias else None
-    ws, nbytes, keep = _scratch(lib.yh_weight_grad_workspace_bytes, dev, rows, n, k)
-    _call(dev, lib.yh_weight_grad, dr.data_ptr(), kind, ldd, qr.data_ptr(), ldq, scale.data_ptr(), rows, n, k,
+    ws, nbytes, keep = _scratch('yh_weight_grad_workspace_bytes', dev, rows, n, k)
+    _call(dev, _abi.load().yh_weight_grad, dr.data_ptr(), kind, ldd, qr.data_ptr(), ldq, scale.data_ptr(), rows, n, k,
           dw.data_ptr(), db.data_ptr() if want_bias else None, ws, nbytes)
     return (dw, db) if want_bias else dw
 
@@ -184,7 +201,7 @@ def weight_grad(dy, codes, scale, want_bias=False):
 def input_grad(dy, w_codes, w_scale):
     """dx [..., K] in dy's type = dy [..., N] times the values of the weight codes [N, K]."""
     dev = _device_of(dy, 'dy')
-    kind = _float_type(dy, 'dy')
+    kind = _float_type(dy.dtype, 'dy')
     dr, rows, n, ldd = _rows(dy, 'dy')
     wr, wn, k, ldw = _codes(w_codes, dev, 'w_codes')
     if w_codes.dim() != 2 or wn != n:
@@ -198,13 +215,38 @@ def input_grad(dy, w_codes, w_scale):
 
 # ------------------------------------------------------------------ normalisation
 class NormKept:
-    """What norm_act leaves for norm_act_backward: `kept` int8 (the activation's side and xhat in seven bits) with
-    a scale for each row, mean and invstd [C] float32, and the call's gamma and slope."""
+    """What norm_act leaves for norm_act_backward: one byte a value (`kept`: the activation's side and xhat in seven
+    bits) with a scale for each row, mean and invstd [C] float32, and the call's gamma and slope.  Everything but gamma
+    lies in one buffer, `store`: rows * pitch bytes, the scales, mean, invstd; the rest are views of it."""
 
-    __slots__ = ('kept', 'scale', 'mean', 'invstd', 'gamma', 'slope')
+    __slots__ = ('store', 'shape', 'rows', 'pitch', 'gamma', 'slope')
 
-    def __init__(self, kept, scale, mean, invstd, gamma, slope):
-        self.kept, self.scale, self.mean, self.invstd, self.gamma, self.slope = kept, scale, mean, invstd, gamma, slope
+    def __init__(self, store, shape, rows, pitch, gamma, slope):
+        self.store, self.shape, self.rows, self.pitch, self.gamma, self.slope = store, shape, rows, pitch, gamma, slope
+
+    def _floats(self, at, n):
+        begin = self.rows * (self.pitch + (4 if self.pitch else 0)) if at else self.rows * self.pitch
+        begin += 4 * self.shape[-1] if at == 2 else 0
+        return self.store[begin:begin + 4 * n].view(torch.float32)
+
+    @property
+    def kept(self):
+        """int8, shaped like z; None if nothing was kept."""
+        if not self.pitch:
+            return None
+        return self.store[:self.rows * self.pitch].view(torch.int8).view(self.shape[:-1] + (self.pitch,))[..., :self.shape[-1]]
+
+    @property
+    def scale(self):
+        return self._floats(0, self.rows).view(self.shape[:-1]) if self.pitch else None
+
+    @property
+    def mean(self):
+        return self._floats(1, self.shape[-1])
+
+    @property
+    def invstd(self):
+        return self._floats(2, self.shape[-1])
 
 
 def norm_act(z, gamma, beta, eps, slope, residual=None, running=None, momentum=0.01, want_kept=True):
@@ -213,8 +255,7 @@ def norm_act(z, gamma, beta, eps, slope, residual=None, running=None, momentum=0
     running: (mean, var) buffers [C], updated in place with `momentum` as torch.nn.BatchNorm2d does (one row
     counts its variance as it is)."""
     dev = _device_of(z, 'z')
-    lib = _abi.load()
-    kind = _float_type(z, 'z')
+    kind = _float_type(z.dtype, 'z')
     zr, rows, c, ldz = _rows(z, 'z')
     gamma, beta = _vector(gamma, c, dev, 'gamma'), _vector(beta, c, dev, 'beta')
     rr, ldr = None, 0
@@ -228,40 +269,39 @@ def norm_act(z, gamma, beta, eps, slope, residual=None, running=None, momentum=0
         for t in (rm, rv):
             if _vector(t, c, dev, 'running').data_ptr() != t.data_ptr():
                 raise ValueError('the running statistics must be contiguous: they are updated in place')
-    a = torch.empty(z.shape, dtype=z.dtype, device=dev)
-    kept = scale = None
-    ldk = 0
-    if want_kept:
-        kept, ldk = _new_codes(tuple(z.shape), dev)
-        scale = torch.empty(z.shape[:-1], dtype=torch.float32, device=dev)
-    stats = torch.empty((2, c), dtype=torch.float32, device=dev)
-    ws, nbytes, keep = _scratch(lib.yh_norm_act_workspace_bytes, dev, rows, c, kind)
-    _call(dev, lib.yh_norm_act_forward, zr.data_ptr(), ldz, None if rr is None else rr.data_ptr(), ldr, kind, rows, c,
-          gamma.data_ptr(), beta.data_ptr(), float(eps), float(slope), a.data_ptr(), c,
-          None if kept is None else kept.data_ptr(), ldk, None if scale is None else scale.data_ptr(),
-          stats.data_ptr(), stats.data_ptr() + 4 * c, None if rm is None else rm.data_ptr(),
-          None if rv is None else rv.data_ptr(), float(momentum), ws, nbytes)
-    return a, NormKept(kept, scale, stats[0], stats[1], gamma, float(slope))
+    shape, slope = tuple(z.shape), float(slope)
+    a = torch.empty(shape, dtype=z.dtype, device=dev)
+    pitch = (c + 15) // 16 * 16 if want_kept else 0
+    head = rows * (pitch + 4) if want_kept else 0
+    store = torch.empty(head + 8 * c, dtype=torch.uint8, device=dev)
+    at = store.data_ptr()
+    ws, nbytes, keep = _scratch('yh_norm_act_workspace_bytes', dev, rows, c, kind)
+    _call(dev, _abi.load().yh_norm_act_forward, zr.data_ptr(), ldz, None if rr is None else rr.data_ptr(), ldr, kind, rows, c,
+          gamma.data_ptr(), beta.data_ptr(), float(eps), slope, a.data_ptr(), c,
+          at if want_kept else None, pitch, at + rows * pitch if want_kept else None, at + head, at + head + 4 * c,
+          None if rm is None else rm.data_ptr(), None if rv is None else rv.data_ptr(), float(momentum), ws, nbytes)
+    return a, NormKept(store, shape, rows, pitch, gamma, slope)
 
 
 def norm_act_backward(da, kept):
     """(dz, dgamma [C], dbeta [C]) of norm_act from a's gradient and the NormKept; the residual's gradient is da."""
     dev = _device_of(da, 'da')
-    lib = _abi.load()
-    kind = _float_type(da, 'da')
-    if kept.kept is None:
+    kind = _float_type(da.dtype, 'da')
+    if not kept.pitch:
         raise ValueError('the forward call kept nothing (want_kept=False)')
-    if da.shape != kept.kept.shape:
-        raise ValueError('da must be shaped like the forward call\'s z, %s, got %s' % (tuple(kept.kept.shape), tuple(da.shape)))
+    if tuple(da.shape) != kept.shape or kept.store.device != dev:
+        raise ValueError('da must be shaped like the forward call\'s z, %s, on %s; got %s' % (kept.shape, kept.store.device, tuple(da.shape)))
     dr, rows, c, ldd = _rows(da, 'da')
-    qr, _, _, ldk = _codes(kept.kept, dev, 'the checkpoint')
-    dz = torch.empty(da.shape, dtype=da.dtype, device=dev)
-    grads = torch.empty((2, c), dtype=torch.float32, device=dev)
-    ws, nbytes, keep = _scratch(lib.yh_norm_act_workspace_bytes, dev, rows, c, kind)
-    _call(dev, lib.yh_norm_act_backward, dr.data_ptr(), ldd, kind, rows, c, qr.data_ptr(), ldk, kept.scale.data_ptr(),
-          kept.gamma.data_ptr(), kept.invstd.data_ptr(), kept.slope, dz.data_ptr(), c,
-          grads.data_ptr(), grads.data_ptr() + 4 * c, ws, nbytes)
-    return dz, grads[0], grads[1]
+    gamma = _vector(kept.gamma, c, dev, 'gamma')
+    dz = torch.empty(kept.shape, dtype=da.dtype, device=dev)
+    dgamma = torch.empty(c, dtype=torch.float32, device=dev)
+    dbeta = torch.empty(c, dtype=torch.float32, device=dev)
+    at = kept.store.data_ptr()
+    scale = at + rows * kept.pitch
+    ws, nbytes, keep = _scratch('yh_norm_act_workspace_bytes', dev, rows, c, kind)
+    _call(dev, _abi.load().yh_norm_act_backward, dr.data_ptr(), ldd, kind, rows, c, at, kept.pitch, scale,
+          gamma.data_ptr(), scale + 4 * rows + 4 * c, kept.slope, dz.data_ptr(), c, dgamma.data_ptr(), dbeta.data_ptr(), ws, nbytes)
+    return dz, dgamma, dbeta
 
 
 # ------------------------------------------------------------------ autograd
@@ -343,15 +383,16 @@ class _NormAct(Function):
     def forward(ctx, z, gamma, beta, eps, slope, residual, running, momentum, keep):
         a, kept = norm_act(z, gamma, beta, eps, slope, residual, running, momentum, want_kept=keep)
         if keep:
-            ctx.save_for_backward(kept.kept, kept.scale, kept.mean, kept.invstd, gamma)
-            ctx.slope = kept.slope
+            ctx.save_for_backward(kept.store, gamma)
+            ctx.layout = kept.shape, kept.rows, kept.pitch, kept.slope
         return a
 
     @staticmethod
     @once_differentiable
     def backward(ctx, da):
-        kept, scale, mean, invstd, gamma = ctx.saved_tensors
-        dz, dgamma, dbeta = norm_act_backward(da, NormKept(kept, scale, mean, invstd, gamma.detach(), ctx.slope))
+        store, gamma = ctx.saved_tensors
+        shape, rows, pitch, slope = ctx.layout
+        dz, dgamma, dbeta = norm_act_backward(da, NormKept(store, shape, rows, pitch, gamma, slope))
         return dz, dgamma, dbeta, None, None, da if ctx.needs_input_grad[5] else None, None, None, None
 
 
