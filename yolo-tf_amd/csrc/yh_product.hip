@@ -1,6 +1,7 @@
 // Products of row codes on the matrix cores: the integer product of a pointwise convolution, and its gradients, which
 // multiply a float matrix by an integer one.
 #include <algorithm>
+#include <type_traits>
 #include "yh_rows.h"
 
 namespace yh {
@@ -73,9 +74,9 @@ __global__ __launch_bounds__(kThreads) void k_int8_tile(const int8_t *x, int64_t
 {
     constexpr int TM = BM / 32, TN = BN / 32;            // 16 x 16 blocks of a wavefront (2 x 2 wavefronts)
     __shared__ __attribute__((aligned(16))) int8_t sx[2][BM * 64], sw[2][BN * 64];
-    const int64_t tile = xcd_run(blockIdx.x, gridDim.x);
-    const int64_t m0 = tile / tiles_n * BM;
-    const int n0 = (int)(tile % tiles_n) * BN;
+    const uint32_t tile = (uint32_t)xcd_run(blockIdx.x, gridDim.x);
+    const int64_t m0 = (int64_t)(tile / (uint32_t)tiles_n) * BM;
+    const int n0 = (int)(tile % (uint32_t)tiles_n) * BN;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
     const int r16 = lane & 15, quad = lane >> 4;
     v4i acc[TN][TM];
@@ -153,199 +154,339 @@ __device__ __forceinline__ uint32_t high_halves(float a, float b)      // the up
 }
 __device__ __forceinline__ float cut8(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-// Eight numbers to three 16-byte chunks of bfloat16.
-__device__ __forceinline__ void split8(const float (&x)[8], v4i (&out)[3])
+// Eight numbers to three operands of bfloat16 numbers.  Two would be enough for the rounding of a 16-bit result, but not
+// for a sum that cancels: what the third holds is up to 2^-16 of every term.
+__device__ __forceinline__ void split8(const float (&x)[8], v8b (&out)[3])
 {
+    uint32_t w[3][4];
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const float r0 = x[i] - cut8(x[i]), r1 = x[i + 1] - cut8(x[i + 1]);
         const float l0 = r0 - cut8(r0), l1 = r1 - cut8(r1);
-        out[0][i / 2] = (int)high_halves(x[i], x[i + 1]);
-        out[1][i / 2] = (int)high_halves(r0, r1);
-        out[2][i / 2] = (int)high_halves(l0, l1);
+        w[0][i / 2] = high_halves(x[i], x[i + 1]);
+        w[1][i / 2] = high_halves(r0, r1);
+        w[2][i / 2] = high_halves(l0, l1);
     }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) __builtin_memcpy(&out[q], w[q], 16);
 }
 
-// The float operand's tile: BA rows (output index) x 32 of the sum.
-// kDown: the sum runs down the rows of dy (weight gradient): a thread takes eight rows of a column, the 64 lanes of a
-//        wavefront neighbouring columns.  Otherwise it runs along a row (input gradient): eight neighbouring numbers.
-template <class T, bool kDown, int BA>
-struct FloatTile {
-    static constexpr int N = BA / 64;
-    float v[N][8], s[8];
-    __device__ __forceinline__ void load(const T *p, int64_t ld, const float *scale, int64_t a0, int64_t na, int64_t r0, int64_t nr)
+// A workgroup's four wavefronts have different rows of the float operand (16 each) and share the integer tile
+// (TB blocks of 16 columns).  A lane's operand is eight numbers along the sum, from (lane >> 4) * 8 on, of output index
+// lane & 15.  The memory pipeline takes neighbouring lanes' addresses together, so every load and store here gives
+// neighbouring lanes neighbouring addresses; what the matrix layout wants otherwise is turned in LDS.
+// Output indexes past the matrix's end read its last row or column again (what they give is not stored), so that a step
+// of 32 whole indexes of the sum asks nothing; offsets are 32 bits from a uniform base (pitches below 2^22: 128 rows of 4-byte elements).
+
+// Loads through a buffer descriptor: a uniform 64-bit base, a uniform 32-bit offset that changes from load to load and a
+// lane offset of 32 bits that does not change at all.  (With plain pointers the compiler keeps and advances one 64-bit
+// address a lane and load, some forty register pairs here.)  The descriptor's bound is the address space's end: every
+// offset is inside of the matrix by construction.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer_at(const void *p)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, -1, 0x00027000);
+}
+__device__ __forceinline__ void load_at(Buffer b, uint32_t lane, uint32_t uniform, uint32_t &v) { v = __builtin_amdgcn_raw_buffer_load_b32(b, lane, uniform, 0); }
+__device__ __forceinline__ void load_at(Buffer b, uint32_t lane, uint32_t uniform, float &v)
+{
+    v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, lane, uniform, 0));
+}
+template <class T>
+__device__ __forceinline__ void load_at(Buffer b, uint32_t lane, uint32_t uniform, T &v)      // 16-bit numbers
+{
+    const uint16_t w = __builtin_amdgcn_raw_buffer_load_b16(b, lane, uniform, 0);
+    __builtin_memcpy(&v, &w, 2);
+}
+__device__ __forceinline__ v4i load_at16(Buffer b, uint32_t lane, uint32_t uniform) { return __builtin_amdgcn_raw_buffer_load_b128(b, lane, uniform, 0); }
+
+// Weight gradient: the sum runs down the rows of dy; a lane takes eight rows of a column straight into its operand, 16
+// lanes 16 neighbouring columns.
+template <class T>
+struct DownOperand {
+    static constexpr int kLds = 0;
+    float v[8];
+    uint32_t off;
+    const T *base;
+    int64_t ld;
+    __device__ __forceinline__ void place(const T *p, int64_t pitch, int64_t a0, int64_t na)
     {
-        if (kDown) {
-            const int64_t r = r0 + (threadIdx.x >> 6) * 8;
+        const int lane = threadIdx.x & 63;
+        const int64_t aw = min(a0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 16, na - 1);
+        base = p + aw;
+        ld = pitch;
+        off = (uint32_t)(((lane >> 4) * 8 * ld + min(aw + (lane & 15), na - 1) - aw) * sizeof(T));
+    }
+    __device__ __forceinline__ void load_whole(int64_t r)
+    {
+        const Buffer p = buffer_at(base + r * ld);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = r + e < nr ? scale[r + e] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int64_t a = a0 + i * 64 + (threadIdx.x & 63);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[i][e] = a < na && r + e < nr ? (float)p[(r + e) * ld + a] : 0.0f;
-            }
-        } else {
-            const int64_t r = r0 + (threadIdx.x & 3) * 8;
-            const int left = (int)min((int64_t)8, nr - r);
-            load_vec<float, 8>(s, scale + r, left);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int64_t a = a0 + i * 64 + (threadIdx.x >> 2);
-                load_vec<T, 8>(v[i], p + a * ld + r, a < na ? left : 0);
-            }
+        for (int e = 0; e < 8; ++e) {
+            T t;
+            load_at(p, off, (uint32_t)(e * ld * sizeof(T)), t);
+            v[e] = (float)t;
         }
     }
-    // the sum of this tile's values in each of the thread's columns (kDown)
-    __device__ __forceinline__ void column_sums(float (&sum)[N]) const
+    __device__ __forceinline__ void load_part(int64_t r, int left)
     {
+        const int k = ((threadIdx.x & 63) >> 4) * 8;
+        const uint32_t a = off - (uint32_t)(k * ld * sizeof(T));                  // the column alone, whatever the pitch
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            sum[i] += ((v[i][0] + v[i][1]) + (v[i][2] + v[i][3])) + ((v[i][4] + v[i][5]) + (v[i][6] + v[i][7]));
+        for (int e = 0; e < 8; ++e) v[e] = k + e < left ? (float)*(base + (r + k + e) * ld + a / sizeof(T)) : 0.0f;
     }
-    __device__ __forceinline__ void store(int8_t *lds) const      // [3][BA] rows of 64 bytes
+    __device__ __forceinline__ void store(int8_t *) const {}
+    __device__ __forceinline__ void fetch(const int8_t *, float (&x)[8]) const
     {
-        const int chunk = kDown ? threadIdx.x >> 6 : threadIdx.x & 3;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int row = i * 64 + (kDown ? threadIdx.x & 63 : threadIdx.x >> 2);
-            float x[8];
-            v4i w[3];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = v[i][e] * s[e];
-            split8(x, w);
-#pragma unroll
-            for (int q = 0; q < 3; ++q) *reinterpret_cast<v4i *>(lds + q * BA * 64 + chunk_at(row, chunk)) = w[q];
-        }
+        for (int e = 0; e < 8; ++e) x[e] = v[e];
     }
 };
 
-// The integer operand's tile: BB columns x 32 of the sum, transposed.  A unit is four columns x four rows of the sum.
-template <int BB>
-struct TurnedTile {
-    uint32_t v[4];
-    __device__ __forceinline__ void load(const int8_t *q, int64_t ld, int b0, int nb, int64_t r0, int64_t nr)
+// Input gradient: the sum runs along the rows of dy.  A tile of 64 rows x 32 goes through LDS as it is, in chunks of 16
+// bytes that sit where eight lanes reading a chunk each of eight rows touch all banks once.
+template <class T>
+struct AlongOperand {
+    static constexpr int E = 16 / (int)sizeof(T), C = 32 / E, N = 64 * C / kThreads, kLds = 64 * C * 16;
+    v4i v[N];
+    uint32_t off[N];
+    const T *base;
+    int64_t ld, a0, na;
+    __device__ __forceinline__ static int place_of(int row, int chunk)
     {
-        const int u = threadIdx.x, b = b0 + (u >> 3) * 4;
-        const int64_t r = r0 + (u & 7) * 4;
+        return row * (C * 16) + ((chunk ^ (C == 8 ? row & 7 : (row >> 1) & 3)) << 4);
+    }
+    __device__ __forceinline__ void place(const T *p, int64_t pitch, int64_t first, int64_t rows)
+    {
+        base = p + first * pitch;
+        ld = pitch, a0 = first, na = rows;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t w[1];
-            load_bytes<4>(w, q + (r + i) * ld + b, (BB * 2 >= kThreads || u < BB * 2) && r + i < nr ? nb - b : 0);
-            v[i] = w[0];
+        for (int n = 0; n < N; ++n) {
+            const int u = threadIdx.x + n * kThreads;
+            off[n] = (uint32_t)((min((int64_t)(u / C), na - 1 - a0) * ld + u % C * E) * sizeof(T));
+        }
+    }
+    __device__ __forceinline__ void load_whole(int64_t r)
+    {
+        const Buffer p = buffer_at(base + r);
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = load_at16(p, off[n], 0);
+    }
+    __device__ __forceinline__ void load_part(int64_t r, int left)
+    {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = threadIdx.x + n * kThreads, c = u % C * E;
+            const T *p = base + min((int64_t)(u / C), na - 1 - a0) * ld + r + c;
+            T w[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = c + e < left ? p[e] : (T)0.0f;
+            __builtin_memcpy(&v[n], w, 16);
         }
     }
     __device__ __forceinline__ void store(int8_t *lds) const
     {
-        const int u = threadIdx.x;
-        if (BB * 2 < kThreads && u >= BB * 2) return;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = (u >> 3) * 4 + j;
-            uint32_t w[2] = {high_halves(code_value(v[0], j), code_value(v[1], j)), high_halves(code_value(v[2], j), code_value(v[3], j))};
-            __builtin_memcpy(__builtin_assume_aligned(lds + chunk_at(row, (u & 7) >> 1) + (u & 1) * 8, 8), w, 8);
+        for (int n = 0; n < N; ++n) {
+            const int u = threadIdx.x + n * kThreads;
+            __builtin_memcpy(__builtin_assume_aligned(lds + place_of(u / C, u % C), 16), &v[n], 16);
         }
     }
-};
-
-// out[a, b] over a tile of BA x BB, sum over [r0, r1).
-template <class T, bool kDown, int BA, int BB>
-struct SplitProduct {
-    static constexpr int TA = BA / 32, TB = BB / 32;
-    v4f acc[TB][TA];
-    __device__ __forceinline__ void step(const int8_t *sa, const int8_t *sb)
+    __device__ __forceinline__ void fetch(const int8_t *lds, float (&x)[8]) const
     {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wa = (wave >> 1) * (BA / 2), wb = (wave & 1) * (BB / 2);
-        v8b b[TB];
+        const int lane = threadIdx.x & 63, row = (threadIdx.x >> 6) * 16 + (lane & 15);
 #pragma unroll
-        for (int i = 0; i < TB; ++i) b[i] = *reinterpret_cast<const v8b *>(sb + chunk_at(wb + i * 16 + (lane & 15), lane >> 4));
+        for (int h = 0; h < 8 / E; ++h) {
+            T t[E];
+            __builtin_memcpy(t, __builtin_assume_aligned(lds + place_of(row, (lane >> 4) * (8 / E) + h), 16), 16);
 #pragma unroll
-        for (int q = 2; q >= 0; --q) {                    // small pieces first
-            v8b a[TA];
-#pragma unroll
-            for (int j = 0; j < TA; ++j) a[j] = *reinterpret_cast<const v8b *>(sa + q * BA * 64 + chunk_at(wa + j * 16 + (lane & 15), lane >> 4));
-#pragma unroll
-            for (int i = 0; i < TB; ++i)
-#pragma unroll
-                for (int j = 0; j < TA; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[i], a[j], acc[i][j], 0, 0, 0);
+            for (int e = 0; e < E; ++e) x[h * E + e] = (float)t[e];
         }
     }
 };
 
-template <class T, bool kDown, int BA, int BB, class TO, bool kSums>
+// The integer operand's tile: BB columns x 32 of the sum, transposed on its way into LDS and made bfloat16 there, once
+// for the four wavefronts.  A unit is four columns x four rows of the sum; the lanes of a row of units read neighbouring
+// words.  Column 4 q + j of the tile becomes LDS row j * BB / 4 + q: the lanes that write column j of their units then
+// write neighbouring rows.  The last columns' unit starts where four are left and shifts them down; units past the end
+// read the last ones.
+template <int BB>
+struct TurnedTile {
+    static constexpr int Q = BB / 4, N = (BB * 2 + kThreads - 1) / kThreads;
+    uint32_t v[N][4], off[N];
+    int shift;
+    __device__ __forceinline__ bool idle() const { return BB * 2 < kThreads && (int)threadIdx.x >= BB * 2; }
+    __device__ __forceinline__ void place(int64_t ld, int left)          // left: columns from the tile's first on, at least 4
+    {
+        const int b = threadIdx.x % Q * 4, c = min(b, left - 4);
+        shift = min(b - c, 3) * 8;
+#pragma unroll
+        for (int n = 0; n < N; ++n) off[n] = (uint32_t)((threadIdx.x + n * kThreads) / Q * 4 * ld + c);
+    }
+    __device__ __forceinline__ void load_whole(const int8_t *base, int64_t ld)
+    {
+        if (idle()) return;
+        const Buffer p = buffer_at(base);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < N; ++n) load_at(p, off[n], (uint32_t)(i * ld), v[n][i]);
+    }
+    __device__ __forceinline__ void load_part(const int8_t *base, int64_t ld, int cols, int left)
+    {
+        if (idle()) return;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int b = threadIdx.x % Q * 4, r = (threadIdx.x + n * kThreads) / Q * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w[1];
+                load_bytes<4>(w, base + (int64_t)(r + i) * ld + b, r + i < left ? cols - b : 0);
+                v[n][i] = w[0] << shift;                             // store() takes it back
+            }
+        }
+    }
+    __device__ __forceinline__ void store(int8_t *lds) const
+    {
+        if (idle()) return;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int q = threadIdx.x % Q, r = (threadIdx.x + n * kThreads) / Q;
+            uint32_t x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = v[n][i] >> shift;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t w[2] = {high_halves(code_value(x[0], j), code_value(x[1], j)), high_halves(code_value(x[2], j), code_value(x[3], j))};
+                __builtin_memcpy(__builtin_assume_aligned(lds + chunk_at(j * Q + q, r >> 1) + (r & 1) * 8, 8), w, 8);
+            }
+        }
+    }
+};
+
+// out[a, b] over 64 x 16 TB values from (a0, b0) on, the sum over [r0, r1) in steps of 32.
+template <class T, bool kDown, int TB, class TO, bool kSums>
 __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float *scale, const int8_t *q, int64_t ldq,
                                            int64_t a0, int64_t na, int b0, int nb, int64_t r0, int64_t r1,
                                            TO *out, int64_t ldo, float *sums)
 {
-    __shared__ __attribute__((aligned(16))) int8_t sa[2][3 * BA * 64], sb[2][BB * 64];
-    SplitProduct<T, kDown, BA, BB> p;
-    constexpr int TA = p.TA, TB = p.TB;
+    typedef typename std::conditional<kDown, DownOperand<T>, AlongOperand<T>>::type Operand;
+    constexpr int BB = 16 * TB, kB = BB * 64, kS = 128, kStage = Operand::kLds + kB + kS;
+    constexpr int kPitch = BB * 4 + 16, kTurn = 4 * 16 * kPitch;      // the results' way out
+    __shared__ __attribute__((aligned(16))) int8_t lds[kTurn > 2 * kStage ? kTurn : 2 * kStage];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    v4f acc[TB];
 #pragma unroll
-    for (int i = 0; i < TB; ++i)
-#pragma unroll
-        for (int j = 0; j < TA; ++j) p.acc[i][j] = v4f{0, 0, 0, 0};
-    FloatTile<T, kDown, BA> ta;
+    for (int i = 0; i < TB; ++i) acc[i] = v4f{0, 0, 0, 0};
+    Operand fa;
     TurnedTile<BB> tb;
-    float col[FloatTile<T, kDown, BA>::N];
+    float scale_v = 0.0f, col = 0.0f;
+    fa.place(dy, ldd, a0, na);
+    tb.place(ldq, max(4, nb - b0));
+    const int8_t *pb = q + b0;
+    const bool near = nb - b0 >= 4 && ldd < (1 << 22) && ldq < (1 << 22);
+    const auto store = [&](int8_t *stage) {
+        fa.store(stage);
+        tb.store(stage + Operand::kLds);
+        if (threadIdx.x < 32) reinterpret_cast<float *>(stage + Operand::kLds + kB)[threadIdx.x] = scale_v;
+    };
+    // the stage's float operand, scaled and split
+    const auto split = [&](const int8_t *stage, v8b (&a)[3]) {
+        float x[8], s[8];
+        fa.fetch(stage, x);
+        __builtin_memcpy(s, __builtin_assume_aligned(stage + Operand::kLds + kB + (lane >> 4) * 32, 16), 32);
+        if (kSums) col += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
-    for (int i = 0; i < ta.N; ++i) col[i] = 0.0f;
-    ta.load(dy, ldd, scale, a0, na, r0, r1);
-    tb.load(q, ldq, b0, nb, r0, r1);
-    ta.store(sa[0]);
-    tb.store(sb[0]);
-    if (kSums) ta.column_sums(col);
-    __syncthreads();
-    int at = 0;
-    for (int64_t r = r0; r < r1; r += 32, at ^= 1) {
-        const bool more = r + 32 < r1;
-        if (more) {
-            ta.load(dy, ldd, scale, a0, na, r + 32, r1);
-            tb.load(q, ldq, b0, nb, r + 32, r1);
+        for (int e = 0; e < 8; ++e) x[e] *= s[e];
+        split8(x, a);
+    };
+    const auto multiply = [&](const int8_t *stage, const v8b (&a)[3]) {
+        // four blocks of columns at a time: an accumulator comes round again after four instructions, not at once
+#pragma unroll
+        for (int i = 0; i < TB; i += 4) {
+            v8b b[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const v8b *>(stage + Operand::kLds + chunk_at((i + c) * 16 + (lane & 15), lane >> 4));
+#pragma unroll
+            for (int p = 2; p >= 0; --p)                              // small pieces first
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[i + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[c], a[p], acc[i + c], 0, 0, 0);
         }
-        p.step(sa[at], sb[at]);
-        if (more) {
-            ta.store(sa[at ^ 1]);
-            tb.store(sb[at ^ 1]);
-            if (kSums) ta.column_sums(col);
+    };
+    int64_t r = r0;
+    int at = 0;
+    const int64_t whole = near ? r0 + (r1 - r0) / 32 * 32 : r0;      // up to here: steps that ask nothing, loaded one ahead
+    if (r < whole) {
+        const auto load = [&](int64_t x) {
+            fa.load_whole(x);
+            tb.load_whole(pb + x * ldq, ldq);
+            if (threadIdx.x < 32) scale_v = scale[x + threadIdx.x];
+        };
+        load(r);
+        store(lds);
+        __syncthreads();
+        for (; r < whole; r += 32, at ^= 1) {
+            const int8_t *stage = lds + at * kStage;
+            v8b a[3];
+            split(stage, a);
+            if (r + 32 < whole) load(r + 32);
+            multiply(stage, a);
+            // the other stage was read in the step before, and every wavefront has passed the barrier since
+            if (r + 32 < whole) store(lds + (at ^ 1) * kStage);
             __syncthreads();
         }
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wa = (wave >> 1) * (BA / 2), wb = (wave & 1) * (BB / 2);
-#pragma unroll
-    for (int j = 0; j < TA; ++j) {
-        const int64_t a = a0 + wa + j * 16 + (lane & 15);
-        if (a >= na) continue;
-#pragma unroll
-        for (int i = 0; i < TB; ++i) {
-            const int b = b0 + wb + i * 16 + (lane >> 4) * 4;
-            float o[4] = {p.acc[i][j][0], p.acc[i][j][1], p.acc[i][j][2], p.acc[i][j][3]};
-            store_vec<TO, 4>(out + a * ldo + b, o, nb - b);
-        }
+    for (; r < r1; r += 32) {
+        const int left = (int)min((int64_t)32, r1 - r);
+        fa.load_part(r, left);
+        tb.load_part(pb + r * ldq, ldq, nb - b0, left);
+        if (threadIdx.x < 32) scale_v = (int)threadIdx.x < left ? scale[r + threadIdx.x] : 0.0f;
+        store(lds);
+        __syncthreads();
+        v8b a[3];
+        split(lds, a);
+        multiply(lds, a);
+        __syncthreads();
     }
-    if (kSums && sums) {                                   // the four wavefronts hold the four eights of every 32 rows
-        __syncthreads();
-        float *f = reinterpret_cast<float *>(sa[0]);
+    // A lane's four rows of LDS order j * BB / 4 + q are four
+    // neighbouring columns of the result; through LDS neighbouring lanes get neighbouring columns of a row.
+    constexpr int H = TB / 4;
+    int8_t *turn = lds + wave * 16 * kPitch;
+    const int64_t first = a0 + wave * 16;
+    if (kSums && sums) {
+        col += __shfl_xor(col, 16);
+        col += __shfl_xor(col, 32);
+        if (lane < 16 && first + lane < na) sums[first + lane] = col;
+    }
 #pragma unroll
-        for (int i = 0; i < ta.N; ++i) f[wave * BA + i * 64 + lane] = col[i];
-        __syncthreads();
-        for (int c = threadIdx.x; c < BA; c += kThreads)
-            if (a0 + c < na) sums[a0 + c] = (f[c] + f[BA + c]) + (f[2 * BA + c] + f[3 * BA + c]);
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v4f o = {acc[h][e], acc[H + h][e], acc[2 * H + h][e], acc[3 * H + h][e]};
+            *reinterpret_cast<v4f *>(turn + (lane & 15) * kPitch + (h * 16 + (lane >> 4) * 4 + e) * 16) = o;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TB; ++i) {
+        const int u = i * 64 + lane, row = u / (BB / 4), b = u % (BB / 4) * 4;
+        float o[4];
+        __builtin_memcpy(o, __builtin_assume_aligned(turn + row * kPitch + b * 4, 16), 16);
+        if (first + row < na && b0 + b < nb) store_vec<TO, 4>(out + (first + row) * ldo + b0 + b, o, nb - b0 - b);
     }
 }
 
 // Weight gradient: workgroup (tile of dw, piece of the rows).  The pieces' results are added by k_add_pieces in a fixed
 // order (no atomics: the same bits on every run).
-template <class T, int BA, int BB>
+template <class T, int TB>
 __global__ __launch_bounds__(kThreads, 2) void k_weight_grad(const T *dy, int64_t ldd, const int8_t *codes, int64_t ldc, const float *scale,
                                                              int64_t rows, int n, int k, int64_t rows_per_piece, int tiles_k, int tiles,
                                                              float *dw, float *db, int64_t pitch)
 {
-    const int64_t id = xcd_run(blockIdx.x, gridDim.x);
-    const int64_t piece = id / tiles;
-    const int tile = (int)(id % tiles), a0 = tile / tiles_k * BA, b0 = tile % tiles_k * BB;
+    const uint32_t id = (uint32_t)xcd_run(blockIdx.x, gridDim.x);
+    const int64_t piece = id / (uint32_t)tiles;
+    const int tile = (int)(id % (uint32_t)tiles), a0 = tile / tiles_k * 64, b0 = tile % tiles_k * 16 * TB;
     const int64_t r0 = piece * rows_per_piece, r1 = min(rows, r0 + rows_per_piece);
-    split_tile<T, true, BA, BB, float, true>(dy, ldd, scale, codes, ldc, a0, n, b0, k, r0, r1,
-                                             dw + piece * pitch, k, db && b0 == 0 ? db + piece * pitch : nullptr);
+    split_tile<T, true, TB, float, true>(dy, ldd, scale, codes, ldc, a0, n, b0, k, r0, r1,
+                                                dw + piece * pitch, k, db && b0 == 0 ? db + piece * pitch : nullptr);
 }
 
 // out[i] = sum of part[p][i] over the pieces, in 64 bits; the first `cut` values are dw, the others db.  A workgroup takes
@@ -375,13 +516,13 @@ __global__ __launch_bounds__(kThreads) void k_fill_zero(float *p, int64_t count)
     if (i < count) p[i] = 0.0f;
 }
 
-template <class T, int BA, int BB>
-__global__ __launch_bounds__(kThreads, 2) void k_input_grad(const T *dy, int64_t ldd, const int8_t *w, int64_t ldw, const float *ws,
+template <class T, int TB>
+__global__ __launch_bounds__(kThreads, 3) void k_input_grad(const T *dy, int64_t ldd, const int8_t *w, int64_t ldw, const float *ws,
                                                             int64_t rows, int n, int k, int tiles_k, T *dx, int64_t lddx)
 {
-    const int64_t tile = xcd_run(blockIdx.x, gridDim.x);
-    split_tile<T, false, BA, BB, T, false>(dy, ldd, ws, w, ldw, tile / tiles_k * BA, rows, (int)(tile % tiles_k) * BB, k, 0, n,
-                                           dx, lddx, nullptr);
+    const uint32_t tile = (uint32_t)xcd_run(blockIdx.x, gridDim.x);
+    split_tile<T, false, TB, T, false>(dy, ldd, ws, w, ldw, (int64_t)(tile / (uint32_t)tiles_k) * 64, rows, (int)(tile % (uint32_t)tiles_k) * 16 * TB, k,
+                                                                   0, n, dx, lddx, nullptr);
 }
 
 template <class F>
@@ -392,16 +533,20 @@ void with_type(int32_t type, F f)
     else f((_Float16)0.0f);
 }
 
-struct GradPlan { int ba, bb, tiles_k, tiles, pieces; int64_t rows_per_piece; };
+// Tiles of 64 ta x 16 tb values: as wide as the result asks, so that the float operand is read and split as seldom as
+// possible.
+// Tiles of 64 x 16 tb values: as wide as the result asks, so that the float operand is read and split as seldom as
+// possible (1024 x 512 weights from 10816 rows: 40 us with tb = 16, 45 us with 8).
+struct GradPlan { int tb, tiles_k, tiles, pieces; int64_t rows_per_piece; };
 GradPlan plan_weight_grad(int64_t rows, int n, int k)
 {
     GradPlan p;
-    p.ba = n <= 64 ? 64 : 128;
-    p.bb = k <= 64 ? 64 : 128;
-    p.tiles_k = (k + p.bb - 1) / p.bb;
-    p.tiles = (n + p.ba - 1) / p.ba * p.tiles_k;
-    // two workgroups a compute unit (their LDS allows no more), each with at least four steps of 32 rows
-    const int64_t want = std::max(1, 2 * 256 / p.tiles), steps = (rows + 31) / 32;
+    p.tb = k <= 64 ? 4 : k <= 128 ? 8 : 16;
+    p.tiles_k = (k + 16 * p.tb - 1) / (16 * p.tb);
+    p.tiles = (n + 63) / 64 * p.tiles_k;
+    // two workgroups a compute unit, each with at least four steps of 32 rows: more pieces cost more in k_add_pieces than
+    // they win (692224 rows, 64 x 128: 64 us in all with 512 workgroups, 65 with 768, 69 with 1024)
+    const int64_t want = std::max(1, 512 / p.tiles), steps = (rows + 31) / 32;
     const int64_t pieces = std::max<int64_t>(1, std::min(want, (steps + 3) / 4));
     p.rows_per_piece = (steps + pieces - 1) / pieces * 32;
     p.pieces = (int)((rows + p.rows_per_piece - 1) / p.rows_per_piece);
@@ -449,12 +594,11 @@ hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, 
     const int64_t pitch = db ? count + n : count;              // a piece: dw, then db
     with_type(dy.type, [&](auto t) {
         using T = decltype(t);
-#define CALL(BA, BB) k_weight_grad<T, BA, BB><<<dim3((unsigned)(p.tiles * p.pieces)), kThreads, 0, st>>>(                   \
+#define CALL(TB) k_weight_grad<T, TB><<<dim3((unsigned)(p.tiles * p.pieces)), kThreads, 0, st>>>(                           \
             static_cast<const T *>(dy.p), dy.ld, codes, ldc, scale, rows, n, k, p.rows_per_piece, p.tiles_k, p.tiles, pw, pb, pitch)
-        if (p.ba == 64 && p.bb == 64) CALL(64, 64);
-        else if (p.ba == 64) CALL(64, 128);
-        else if (p.bb == 64) CALL(128, 64);
-        else CALL(128, 128);
+        if (p.tb == 4) CALL(4);
+        else if (p.tb == 8) CALL(8);
+        else CALL(16);
 #undef CALL
     });
     if (p.pieces > 1) {
@@ -472,15 +616,15 @@ hipError_t launch_input_grad(const Rows &dy, const int8_t *w, int64_t ldw, const
     (void)type;
     with_type(dy.type, [&](auto t) {
         using T = decltype(t);
-#define CALL(BA, BB)                                                                                                        \
+#define CALL(TB)                                                                                                            \
         do {                                                                                                                \
-            const int tk = (k + BB - 1) / BB;                                                                               \
-            k_input_grad<T, BA, BB><<<dim3((unsigned)((rows + BA - 1) / BA * tk)), kThreads, 0, st>>>(                      \
+            const int tk = (k + 16 * TB - 1) / (16 * TB);                                                                   \
+            k_input_grad<T, TB><<<dim3((unsigned)((rows + 63) / 64 * tk)), kThreads, 0, st>>>(                              \
                 static_cast<const T *>(dy.p), dy.ld, w, ldw, w_scale, rows, n, k, tk, static_cast<T *>(dx), lddx);          \
         } while (0)
-        if (k <= 64) CALL(64, 64);
-        else if ((rows + 127) / 128 * ((k + 127) / 128) >= 256) CALL(128, 128);
-        else CALL(64, 64);
+        // (43264 rows, 256 -> 512: 40 us with 8, 45 with 16, 51 with 4); half as wide where that gives too few workgroups
+        if (k > 64 && (rows + 63) / 64 * ((k + 127) / 128) >= 256) CALL(8);
+        else CALL(4);
 #undef CALL
     });
     return hipGetLastError();
