@@ -86,9 +86,10 @@ def test_refusals_of_the_products():
     _refused(m(ws=None), inv, 'w_scale is null')
     _refused(m(b=0x7002), ali, 'bias')
     _refused(m(ldy=4), inv, 'y: 4')
-    _refused(m(work=None), wsp, 'workspace')
-    _refused(m(size=79), wsp, 'workspace')
-    _refused(m(work=0x5008), ali, 'workspace')
+    wide = dict(rows=5000, k=5000, ldx=5000, ldw=5000)               # a size whose codes pass through a workspace
+    _refused(m(work=None, **wide), wsp, 'workspace')
+    _refused(m(size=5000 * 5000 - 1, **wide), wsp, 'workspace')
+    _refused(m(work=0x5008, size=1 << 30, **wide), ali, 'workspace')
     _refused(m(k=1 << 16, n=1 << 16), lim, 'weights')
     _refused(m(rows=(1 << 26) - 1, k=1 << 15), lim, '2^38')
     assert m(rows=0) == _abi.YH_OK
@@ -152,9 +153,12 @@ def test_workspace_sizes():
     lib = _abi.load()
     n = ctypes.c_size_t(7)
     ask = lambda fn, *a: (_abi.check(fn(*a, ctypes.byref(n))), n.value)[1]
-    assert ask(lib.yh_matmul_int8_workspace_bytes, 100, 33, 5, F32, 0) >= 100 * (48 + 4)
-    assert ask(lib.yh_matmul_int8_workspace_bytes, 100, 33, 5, F32, 1) == 0
-    assert ask(lib.yh_matmul_int8_workspace_bytes, 100, 33, 5, I8, 0) == 0
+    # zero, or the codes and their scales
+    for rows, k, n_out in ((1, 1, 1), (100, 33, 5), (5000, 5000, 500), (173056, 256, 128), (43264, 1536, 425), (60000, 1000, 1000)):
+        assert ask(lib.yh_matmul_int8_workspace_bytes, rows, k, n_out, F32, 0) in (0, rows * ((k + 15) // 16 * 16 + 4))
+        assert ask(lib.yh_matmul_int8_workspace_bytes, rows, k, n_out, F32, 1) == 0
+        assert ask(lib.yh_matmul_int8_workspace_bytes, rows, k, n_out, I8, 0) == 0
+    assert ask(lib.yh_matmul_int8_workspace_bytes, 5000, 5000, 500, F32, 0) > 0
     assert ask(lib.yh_weight_grad_workspace_bytes, 0, 64, 64) == 0
     # the pieces of the rows never take more than their number times the result, and that number is bounded
     for rows, a, b in ((1, 1, 1), (700000, 64, 128), (10816, 512, 1024), (50000, 1536, 1536)):

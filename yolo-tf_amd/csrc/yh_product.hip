@@ -24,6 +24,28 @@ __device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t total)
 // (or write) one chunk each of eight neighbouring rows touch all 32 banks once.
 __device__ __forceinline__ int chunk_at(int row, int chunk) { return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4); }
 
+// Loads through a buffer descriptor: a uniform 64-bit base, a uniform 32-bit offset that changes from load to load and a
+// lane offset of 32 bits that does not change at all.  (With plain pointers the compiler keeps and advances one 64-bit
+// address a lane and load, some forty register pairs here.)  The descriptor's bound is the address space's end: every
+// offset is inside of the matrix by construction.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer_at(const void *p)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, -1, 0x00027000);
+}
+__device__ __forceinline__ void load_at(Buffer b, uint32_t lane, uint32_t uniform, uint32_t &v) { v = __builtin_amdgcn_raw_buffer_load_b32(b, lane, uniform, 0); }
+__device__ __forceinline__ void load_at(Buffer b, uint32_t lane, uint32_t uniform, float &v)
+{
+    v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, lane, uniform, 0));
+}
+template <class T>
+__device__ __forceinline__ void load_at(Buffer b, uint32_t lane, uint32_t uniform, T &v)      // 16-bit numbers
+{
+    const uint16_t w = __builtin_amdgcn_raw_buffer_load_b16(b, lane, uniform, 0);
+    __builtin_memcpy(&v, &w, 2);
+}
+__device__ __forceinline__ v4i load_at16(Buffer b, uint32_t lane, uint32_t uniform) { return __builtin_amdgcn_raw_buffer_load_b128(b, lane, uniform, 0); }
+
 // ---- y = (codes . w codes^T) * scale * w_scale + bias ---------------------
 // The sums are whole numbers in 32 bits (exact up to 65536 terms of 127^2); one product by each scale in float32 and one
 // rounding to the output's type follow.  The weights are the matrix instruction's first operand: a lane then holds four
@@ -45,16 +67,34 @@ __device__ __forceinline__ v4i load_chunk(const int8_t *p, int left)
     return v;
 }
 
+// R rows x 64 of the sum.  Rows past the matrix's end read its last row again (their results are not stored), so that a
+// whole step asks nothing; load_part() reads what is left of the sum and zeros behind it.
 template <int R>
 struct CodeTile {
-    static constexpr int N = (R * 4 + kThreads - 1) / kThreads;
+    static constexpr int N = R * 4 / kThreads;
     v4i v[N];
-    __device__ __forceinline__ void load(const int8_t *p, int64_t ld, int64_t row0, int64_t rows, int k0, int k)
+    uint32_t off[N];
+    const int8_t *base;
+    int64_t ld, last;
+    __device__ __forceinline__ void place(const int8_t *p, int64_t pitch, int64_t row0, int64_t rows)
+    {
+        base = p + row0 * pitch;
+        ld = pitch, last = rows - 1 - row0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) off[i] = (uint32_t)(min((int64_t)(threadIdx.x + i * kThreads) >> 2, last) * ld + (threadIdx.x & 3) * 16);
+    }
+    __device__ __forceinline__ void load_whole(int k0)
+    {
+        const Buffer b = buffer_at(base + k0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = load_at16(b, off[i], 0);
+    }
+    __device__ __forceinline__ void load_part(int k0, int k)
     {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int u = threadIdx.x + i * kThreads, r = u >> 2, c = k0 + (u & 3) * 16;
-            v[i] = load_chunk(p + (row0 + r) * ld + c, (R * 4 >= kThreads || u < R * 4) && row0 + r < rows ? k - c : 0);
+            const int c = k0 + (threadIdx.x & 3) * 16;
+            v[i] = load_chunk(base + min((int64_t)(threadIdx.x + i * kThreads) >> 2, last) * ld + c, k - c);
         }
     }
     __device__ __forceinline__ void store(int8_t *lds) const
@@ -62,77 +102,409 @@ struct CodeTile {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int u = threadIdx.x + i * kThreads;
-            if (R * 4 >= kThreads || u < R * 4) *reinterpret_cast<v4i *>(lds + chunk_at(u >> 2, u & 3)) = v[i];
+            *reinterpret_cast<v4i *>(lds + chunk_at(u >> 2, u & 3)) = v[i];
         }
     }
 };
+
+// Orders a wavefront's LDS writes before its other lanes' reads.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int kOutPitch = 64 * 4 + 16;                     // 16 rows of 64 results on their way out of a wavefront
+
+// 16 x 64 results of a wavefront: scaled, in LDS with neighbouring columns together, out.  acc[i] holds channels
+// n0 + 16 i + 4 (lane >> 4) + 0..3 of row lane & 15.
+template <class T>
+__device__ __forceinline__ void out_16x64(const v4i (&acc)[4], float s, const float *ws, const float *bias, int8_t *turn,
+                                          T *y, int64_t ldy, int64_t first, int64_t rows, int n0, int n)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = i * 16 + (lane >> 4) * 4;
+        v4f o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (float)acc[i][e] * s * ws[c + e] + bias[c + e];
+        *reinterpret_cast<v4f *>(turn + (lane & 15) * kOutPitch + c * 4) = o;
+    }
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 4 + (lane >> 4), c = (lane & 15) * 4;
+        float o[4];
+        __builtin_memcpy(o, __builtin_assume_aligned(turn + row * kOutPitch + c * 4, 16), 16);
+        if (first + row < rows) store_vec<T, 4>(y + (first + row) * ldy + n0 + c, o, n - n0 - c);
+    }
+    wave_sync();
+}
 
 template <class T, int BM, int BN>
 __global__ __launch_bounds__(kThreads) void k_int8_tile(const int8_t *x, int64_t ldx, const float *xs, int64_t rows, int k,
                                                         const int8_t *w, int64_t ldw, const float *ws, int n, const float *bias,
                                                         T *y, int64_t ldy, int tiles_n)
 {
-    constexpr int TM = BM / 32, TN = BN / 32;            // 16 x 16 blocks of a wavefront (2 x 2 wavefronts)
-    __shared__ __attribute__((aligned(16))) int8_t sx[2][BM * 64], sw[2][BN * 64];
+    constexpr int WN = BN / 64, WM = 4 / WN, TM = BM / WM / 16, TN = 4;       // wavefronts of 64 channels, 16 x 16 blocks of one
+    constexpr int kStage = (BM + BN) * 64, kTurn = 4 * 16 * kOutPitch;
+    __shared__ __attribute__((aligned(16))) int8_t lds[2 * kStage > kTurn ? 2 * kStage : kTurn];
+    __shared__ float lsc[BN], lb[BN];
     const uint32_t tile = (uint32_t)xcd_run(blockIdx.x, gridDim.x);
     const int64_t m0 = (int64_t)(tile / (uint32_t)tiles_n) * BM;
     const int n0 = (int)(tile % (uint32_t)tiles_n) * BN;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN * (BM / WM), wn = wave % WN * 64;
     const int r16 = lane & 15, quad = lane >> 4;
-    v4i acc[TN][TM];
+    for (int u = threadIdx.x; u < BN; u += kThreads) {
+        lsc[u] = n0 + u < n ? ws[n0 + u] : 0.0f;
+        lb[u] = bias && n0 + u < n ? bias[n0 + u] : 0.0f;
+    }
+    v4i acc[TM][TN];
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
+    for (int j = 0; j < TM; ++j)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+        for (int i = 0; i < TN; ++i) acc[j][i] = v4i{0, 0, 0, 0};
     CodeTile<BM> tx;
     CodeTile<BN> tw;
-    const int steps = (k + 63) / 64;
-    tx.load(x, ldx, m0, rows, 0, k);
-    tw.load(w, ldw, n0, n, 0, k);
-    tx.store(sx[0]);
-    tw.store(sw[0]);
-    __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        const int at = s & 1;
-        if (s + 1 < steps) {
-            tx.load(x, ldx, m0, rows, (s + 1) * 64, k);
-            tw.load(w, ldw, n0, n, (s + 1) * 64, k);
-        }
+    tx.place(x, ldx, m0, rows);
+    tw.place(w, ldw, n0, n);
+    const auto store = [&](int8_t *stage) {
+        tx.store(stage);
+        tw.store(stage + BM * 64);
+    };
+    const auto multiply = [&](const int8_t *sx) {
+        const int8_t *sw = sx + BM * 64;
         v4i a[TN], b[TM];
 #pragma unroll
-        for (int i = 0; i < TN; ++i) a[i] = *reinterpret_cast<const v4i *>(sw[at] + chunk_at(wn + i * 16 + r16, quad));
+        for (int i = 0; i < TN; ++i) a[i] = *reinterpret_cast<const v4i *>(sw + chunk_at(wn + i * 16 + r16, quad));
 #pragma unroll
-        for (int j = 0; j < TM; ++j) b[j] = *reinterpret_cast<const v4i *>(sx[at] + chunk_at(wm + j * 16 + r16, quad));
+        for (int j = 0; j < TM; ++j) b[j] = *reinterpret_cast<const v4i *>(sx + chunk_at(wm + j * 16 + r16, quad));
 #pragma unroll
-        for (int i = 0; i < TN; ++i)
+        for (int j = 0; j < TM; ++j)
 #pragma unroll
-            for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], b[j], acc[i][j], 0, 0, 0);
-        if (s + 1 < steps) {
-            tx.store(sx[at ^ 1]);
-            tw.store(sw[at ^ 1]);
-            __syncthreads();
+            for (int i = 0; i < TN; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], b[j], acc[j][i], 0, 0, 0);
+    };
+    const int whole = ldx < (1 << 22) && ldw < (1 << 22) ? k & ~63 : 0;
+    if (whole) {
+        tx.load_whole(0);
+        tw.load_whole(0);
+        store(lds);
+        __syncthreads();
+    }
+    int at = 0;
+    for (int q = 0; q < whole; q += 64, at ^= 1) {
+        if (q + 64 < whole) {
+            tx.load_whole(q + 64);
+            tw.load_whole(q + 64);
         }
+        multiply(lds + at * kStage);
+        // the other stage was read in the step before, and every wavefront has passed the barrier since
+        if (q + 64 < whole) store(lds + (at ^ 1) * kStage);
+        __syncthreads();
+    }
+    for (int q = whole; q < k; q += 64) {
+        tx.load_part(q, k);
+        tw.load_part(q, k);
+        store(lds);
+        __syncthreads();
+        multiply(lds);
+        __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-        const int c = n0 + wn + i * 16 + quad * 4;
-        float sc[4], bi[4];
-        load_vec<float, 4>(sc, ws + c, n - c);
-        if (bias) load_vec<float, 4>(bi, bias + c, n - c);
+    for (int j = 0; j < TM; ++j) {
+        const int64_t r = m0 + wm + j * 16;
+        out_16x64<T>(acc[j], r + r16 < rows ? xs[r + r16] : 0.0f, lsc + wn, lb + wn, lds + wave * 16 * kOutPitch, y, ldy, r, rows, n0 + wn, n);
+    }
+}
+
+// 16 bytes of a row's elements from p on, `left` of them inside of the row; zeros behind.
+template <class TX, bool kWhole>
+__device__ __forceinline__ v4i load_elements(const TX *p, int left)
+{
+    constexpr int V = 16 / (int)sizeof(TX);
+    v4i v = {0, 0, 0, 0};
+    if (left >= V) {
+        const LooseBytes<16>::type t = *reinterpret_cast<const LooseBytes<16>::type *>(p);
+        __builtin_memcpy(&v, &t, 16);
+    } else if (!kWhole && left > 0) {
+        TX t[V];
 #pragma unroll
-        for (int j = 0; j < TM; ++j) {
-            const int64_t r = m0 + wm + j * 16 + r16;
-            if (r >= rows) continue;
-            const float s = xs[r];
-            float o[4];
+        for (int i = 0; i < V; ++i) t[i] = i < left ? p[i] : (TX)0;
+        __builtin_memcpy(&v, t, 16);
+    }
+    return v;
+}
+
+// ---- the same from float rows: codes taken on the way --------------------------
+// Reading x once and writing y once is all the product has to move, so where it can the product takes the codes itself
+// and they stay in LDS.  A wavefront turns 16 rows into codes at a time: `lanes` (4 to 16) neighbouring lanes a row, four
+// vectors of 16 bytes each, so rows of up to 1024 bytes, and leaves them in LDS rows of k64 + 16 bytes (k64: K rounded up to 64, zeros
+// behind K; the 16 bytes shift each row by a bank group, so that 16 rows are read without a conflict).
+template <class TX, int G, bool kWhole>                  // kWhole: K is a multiple of V
+struct CodeRows {
+    static constexpr int V = 16 / (int)sizeof(TX);
+    v4i raw[G][4];                                       // G = lanes / 4 passes of 64 / lanes rows, as they are in memory
+    const TX *x;
+    int64_t ldx, rows;
+    int k, k64, lanes;
+    __device__ __forceinline__ void load(int64_t first)
+    {
+        const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), per = 64 / lanes;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o[e] = (float)acc[i][j][e] * s * sc[e];
-                if (bias) o[e] += bi[e];
+        for (int g = 0; g < G; ++g) {
+            const int64_t row = first + g * per + lane / lanes;
+            const TX *p = x + row * ldx;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = (i * lanes + sub) * V;
+                raw[g][i] = load_elements<TX, kWhole>(p + c, row < rows ? k - c : 0);
             }
-            store_vec<T, 4>(y + r * ldy + c, o, n - c);
         }
     }
+    // what is loaded, the 16 rows from `first` on, as codes to `lds` and scales to `ls`, and to codes / scale if they are
+    // not null
+    __device__ __forceinline__ void put(int64_t first, int8_t *lds, float *ls, int8_t *codes, int64_t ldc, float *scale) const
+    {
+        const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), per = 64 / lanes;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int r = g * per + lane / lanes;
+            float v[4][V];
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                TX t[V];
+                __builtin_memcpy(t, &raw[g][i], 16);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    v[i][j] = (float)t[j];
+                    m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
+                }
+            }
+            const RowScale s = row_scale(row_max(m, lanes), (float)kCodeMax);
+            const bool in = first + r < rows;
+            if (sub == 0) {
+                ls[r] = s.s;
+                if (scale && in) scale[first + r] = s.s;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = (i * lanes + sub) * V;
+                uint32_t w[V / 4];
+#pragma unroll
+                for (int j = 0; j < V; j += 4) {
+                    const uint32_t q = pack4(code_bits(v[i][j], s.r), code_bits(v[i][j + 1], s.r), code_bits(v[i][j + 2], s.r), code_bits(v[i][j + 3], s.r));
+                    w[j / 4] = s.live ? q : 0u;
+                }
+                if (c < k64) __builtin_memcpy(__builtin_assume_aligned(lds + r * (k64 + 16) + c, V), w, V);
+                if (codes && in) store_bytes<V>(codes + (first + r) * ldc + c, w, k - c);
+            }
+        }
+    }
+};
+template <int G, bool kWhole>
+struct CodeRows<int8_t, G, kWhole> {                     // codes already
+    static constexpr int V = 16;
+    v4i raw[G][4];
+    const int8_t *x;
+    int64_t ldx, rows;
+    int k, k64, lanes;
+    __device__ __forceinline__ void load(int64_t first)
+    {
+        const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), per = 64 / lanes;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t row = first + g * per + lane / lanes;
+                const int c = (i * lanes + sub) * V;
+                raw[g][i] = load_elements<int8_t, kWhole>(x + row * ldx + c, row < rows ? k - c : 0);
+            }
+    }
+    __device__ __forceinline__ void put(int64_t, int8_t *lds, float *, int8_t *, int64_t, float *) const
+    {
+        const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), per = 64 / lanes;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = (i * lanes + sub) * V;
+                if (c < k64) *reinterpret_cast<v4i *>(lds + (g * per + lane / lanes) * (k64 + 16) + c) = raw[g][i];
+            }
+    }
+};
+
+// Many rows, weights that fit: a workgroup keeps all weights in LDS for good and its eight wavefronts, which have nothing
+// more to say to each other, take blocks of 16 rows in turn, the next block's loads under this block's arithmetic.  Bound
+// by memory: 173056 rows, 256 -> 128 in float32 move 266 MB in 59 us (4.5 TB/s), 692224 rows, 128 -> 64 532 MB in 110 us
+// (4.8 TB/s); through codes in memory they take 77 and 179 us.
+constexpr int kRowWaves = 8;
+
+template <class TX, class T, int G, bool kWhole>
+__global__ __launch_bounds__(64 * kRowWaves) void k_int8_rows(const TX *x, int64_t ldx, const float *xs, int64_t rows, int k, int lanes,
+                                                   const int8_t *w, int64_t ldw, const float *ws, int n, const float *bias,
+                                                   T *y, int64_t ldy, int8_t *codes, int64_t ldc, float *scale)
+{
+    extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+    const int k64 = (k + 63) / 64 * 64, pitch = k64 + 16, nw = (n + 63) / 64 * 64;
+    int8_t *lw = lds;
+    float *lsc = reinterpret_cast<float *>(lds + nw * pitch), *lb = lsc + nw;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int8_t *mine = reinterpret_cast<int8_t *>(lb + nw) + wave * (16 * pitch + 16 * kOutPitch + 64);
+    int8_t *lx = mine, *turn = mine + 16 * pitch;
+    float *ls = reinterpret_cast<float *>(turn + 16 * kOutPitch);
+    const int per = k64 / 16;
+    for (int u = threadIdx.x; u < nw * per; u += blockDim.x) {
+        const int r = u / per, c = (u - r * per) * 16;
+        *reinterpret_cast<v4i *>(lw + r * pitch + c) = load_chunk(w + (int64_t)r * ldw + c, r < n ? k - c : 0);
+    }
+    for (int u = threadIdx.x; u < nw; u += blockDim.x) {
+        lsc[u] = u < n ? ws[u] : 0.0f;
+        lb[u] = bias && u < n ? bias[u] : 0.0f;
+    }
+    __syncthreads();
+    CodeRows<TX, G, kWhole> in;
+    in.x = x, in.ldx = ldx, in.rows = rows, in.k = k, in.k64 = k64, in.lanes = lanes;
+    const int64_t stride = (int64_t)gridDim.x * kRowWaves;
+    int64_t b = (int64_t)blockIdx.x * kRowWaves + wave;
+    if (b * 16 < rows) in.load(b * 16);
+    for (; b * 16 < rows; b += stride) {
+        in.put(b * 16, lx, ls, codes, ldc, scale);
+        in.load((b + stride) * 16);                        // under this block's products
+        wave_sync();
+        const float s = sizeof(TX) == 1 ? (b * 16 + (lane & 15) < rows ? xs[b * 16 + (lane & 15)] : 0.0f) : ls[lane & 15];
+        const int at = (lane & 15) * pitch + (lane >> 4) * 16;
+        for (int c0 = 0; c0 < nw; c0 += 64) {
+            v4i acc[4] = {};
+            for (int q = 0; q < k64; q += 64) {
+                const v4i xv = *reinterpret_cast<const v4i *>(lx + at + q);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i *>(lw + (c0 + i * 16) * pitch + at + q), xv, acc[i], 0, 0, 0);
+            }
+            out_16x64<T>(acc, s, lsc + c0, lb + c0, turn, y, ldy, b * 16, rows, c0, n);
+        }
+    }
+}
+
+// Four rows of a workgroup's 16 a wavefront, each by all its lanes: codes at lx, scales at ls (k_int8_few).
+template <class TX, bool kWhole>
+__device__ __forceinline__ void code_four_rows(const TX *x, int64_t ldx, const float *, int64_t first, int64_t rows, int k, int k64,
+                                               int8_t *lx, float *ls, int8_t *codes, int64_t ldc, float *scale)
+{
+    constexpr int V = RowVec<TX>::V, IT = 4;
+    const int lane = threadIdx.x & 63, r0 = (threadIdx.x >> 6) * 4, pitch = k64 + 16;
+    const bool once = k <= IT * 64 * V;                    // the row fits the wavefront's registers
+    v4i raw[4][IT];
+    uint32_t m[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = (i * 64 + lane) * V;
+            raw[r][i] = load_elements<TX, kWhole>(x + (first + r0 + r) * ldx + c, first + r0 + r < rows ? k - c : 0);
+        }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        float v[IT][V];
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            TX t[V];
+            __builtin_memcpy(t, &raw[r][i], 16);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[i][j] = (float)t[j];
+                m[r] = max(m[r], __float_as_uint(v[i][j]) & 0x7fffffffu);
+            }
+        }
+        if (!once && first + r0 + r < rows)
+            for (int c = (IT * 64 + lane) * V; c < k; c += 64 * V) {
+                float t[V];
+                load_vec<TX, V>(t, x + (first + r0 + r) * ldx + c, k - c);
+#pragma unroll
+                for (int j = 0; j < V; ++j) m[r] = max(m[r], __float_as_uint(t[j]) & 0x7fffffffu);
+            }
+        const RowScale s = row_scale(row_max(m[r], 64), (float)kCodeMax);
+        const bool in = first + r0 + r < rows;
+        if (lane == 0) {
+            ls[r0 + r] = s.s;
+            if (scale && in) scale[first + r0 + r] = s.s;
+        }
+        const auto put = [&](const float (&t)[V], int c) {
+            uint32_t w[V / 4];
+#pragma unroll
+            for (int j = 0; j < V; j += 4) {
+                const uint32_t q = pack4(code_bits(t[j], s.r), code_bits(t[j + 1], s.r), code_bits(t[j + 2], s.r), code_bits(t[j + 3], s.r));
+                w[j / 4] = s.live ? q : 0u;
+            }
+            if (c < k64) __builtin_memcpy(__builtin_assume_aligned(lx + (r0 + r) * pitch + c, V), w, V);
+            if (codes && in) store_bytes<V>(codes + (first + r0 + r) * ldc + c, w, k - c);
+        };
+#pragma unroll
+        for (int i = 0; i < IT; ++i) put(v[i], (i * 64 + lane) * V);
+        if (!once)
+            for (int c = (IT * 64 + lane) * V; c < k64; c += 64 * V) {
+                float t[V];
+                load_vec<TX, V>(t, x + (first + r0 + r) * ldx + c, in ? k - c : 0);
+                put(t, c);
+            }
+    }
+}
+template <bool kWhole>
+__device__ __forceinline__ void code_rows_given(const int8_t *x, int64_t ldx, const float *xs, int64_t first, int64_t rows, int k, int k64, int8_t *lx, float *ls)
+{
+    const int per = k64 / 16;
+    if (threadIdx.x < 16) ls[threadIdx.x] = first + threadIdx.x < rows ? xs[first + threadIdx.x] : 0.0f;
+    for (int u = threadIdx.x; u < 16 * per; u += kThreads) {
+        const int r = u / per, c = (u - r * per) * 16;
+        *reinterpret_cast<v4i *>(lx + r * (k64 + 16) + c) = load_elements<int8_t, kWhole>(x + (first + r) * ldx + c, first + r < rows ? k - c : 0);
+    }
+}
+
+// Few rows: a workgroup takes 16 rows and 64 channels, 16 a wavefront.  The weights' loads are under way before the rows
+// are turned into codes (four rows a wavefront); nothing is read in turns, so a call lasts about three memory latencies.
+template <class TX, class T, bool kWhole>
+__global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx, const float *xs, int64_t rows, int k,
+                                                       const int8_t *w, int64_t ldw, const float *ws, int n, const float *bias,
+                                                       T *y, int64_t ldy, int8_t *codes, int64_t ldc, float *scale)
+{
+    constexpr int kAhead = 16;                             // steps of 64 whose weights are fetched first
+    extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+    const int k64 = (k + 63) / 64 * 64, pitch = k64 + 16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, quad = lane >> 4;
+    const int64_t first = (int64_t)blockIdx.x * 16;
+    const int n0 = blockIdx.y * 64 + wave * 16;
+    int8_t *lx = lds;
+    float *ls = reinterpret_cast<float *>(lds + 16 * pitch);
+    const int8_t *wr = w + (int64_t)min(n0 + r16, n - 1) * ldw;
+    v4i a[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) a[i] = load_elements<int8_t, kWhole>(wr + i * 64 + quad * 16, k - i * 64 - quad * 16);
+    if (blockIdx.y) codes = nullptr, scale = nullptr;
+    if constexpr (sizeof(TX) == 1) code_rows_given<kWhole>(x, ldx, xs, first, rows, k, k64, lx, ls);
+    else code_four_rows<TX, kWhole>(x, ldx, xs, first, rows, k, k64, lx, ls, codes, ldc, scale);
+    __syncthreads();
+    v4i acc = {0, 0, 0, 0};
+    const int8_t *at = lx + r16 * pitch + quad * 16;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (i * 64 < k64) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], *reinterpret_cast<const v4i *>(at + i * 64), acc, 0, 0, 0);
+    for (int q = kAhead * 64; q < k64; q += 64)
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_elements<int8_t, kWhole>(wr + q + quad * 16, k - q - quad * 16), *reinterpret_cast<const v4i *>(at + q), acc, 0, 0, 0);
+    const int64_t row = first + r16;
+    const int c = n0 + quad * 4;
+    if (row >= rows) return;
+    const float s = ls[r16];
+    float sc[4], bi[4], o[4];
+    load_vec<float, 4>(sc, ws + c, n - c);
+    if (bias) load_vec<float, 4>(bi, bias + c, n - c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        o[e] = (float)acc[e] * s * sc[e];
+        if (bias) o[e] += bi[e];
+    }
+    store_vec<T, 4>(y + row * ldy + c, o, n - c);
 }
 
 // ---- float x integer products ---------------------------------------------
@@ -177,28 +549,6 @@ __device__ __forceinline__ void split8(const float (&x)[8], v8b (&out)[3])
 // neighbouring lanes neighbouring addresses; what the matrix layout wants otherwise is turned in LDS.
 // Output indexes past the matrix's end read its last row or column again (what they give is not stored), so that a step
 // of 32 whole indexes of the sum asks nothing; offsets are 32 bits from a uniform base (pitches below 2^22: 128 rows of 4-byte elements).
-
-// Loads through a buffer descriptor: a uniform 64-bit base, a uniform 32-bit offset that changes from load to load and a
-// lane offset of 32 bits that does not change at all.  (With plain pointers the compiler keeps and advances one 64-bit
-// address a lane and load, some forty register pairs here.)  The descriptor's bound is the address space's end: every
-// offset is inside of the matrix by construction.
-typedef __amdgpu_buffer_rsrc_t Buffer;
-__device__ __forceinline__ Buffer buffer_at(const void *p)
-{
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, -1, 0x00027000);
-}
-__device__ __forceinline__ void load_at(Buffer b, uint32_t lane, uint32_t uniform, uint32_t &v) { v = __builtin_amdgcn_raw_buffer_load_b32(b, lane, uniform, 0); }
-__device__ __forceinline__ void load_at(Buffer b, uint32_t lane, uint32_t uniform, float &v)
-{
-    v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, lane, uniform, 0));
-}
-template <class T>
-__device__ __forceinline__ void load_at(Buffer b, uint32_t lane, uint32_t uniform, T &v)      // 16-bit numbers
-{
-    const uint16_t w = __builtin_amdgcn_raw_buffer_load_b16(b, lane, uniform, 0);
-    __builtin_memcpy(&v, &w, 2);
-}
-__device__ __forceinline__ v4i load_at16(Buffer b, uint32_t lane, uint32_t uniform) { return __builtin_amdgcn_raw_buffer_load_b128(b, lane, uniform, 0); }
 
 // Weight gradient: the sum runs down the rows of dy; a lane takes eight rows of a column straight into its operand, 16
 // lanes 16 neighbouring columns.
@@ -557,21 +907,108 @@ unsigned blocks_for(int64_t count) { return (unsigned)((count + kThreads - 1) / 
 
 }  // namespace
 
-hipError_t launch_int8_product(const int8_t *x, int64_t ldx, const float *x_scale, int64_t rows, int32_t k,
-                               const int8_t *w, int64_t ldw, const float *w_scale, int32_t n, const float *bias,
-                               void *y, int64_t ldy, int32_t type, hipStream_t st)
+namespace {
+
+int pow2_at_least(int v)
 {
+    int p = 1;
+    while (p < v) p <<= 1;
+    return p;
+}
+
+// How a product is computed.  All three give the same bits: the sums are whole numbers.
+struct ProductPlan {
+    enum { kTile, kRows, kFew } how;
+    int lanes;                                           // kRows: of a row
+    size_t lds;
+};
+ProductPlan plan_product(int64_t rows, int k, int n, int x_type)
+{
+    ProductPlan p{};
+    const int k64 = (k + 63) / 64 * 64, n64 = (n + 63) / 64 * 64, V = x_type == YH_INT8 ? 16 : x_type == YH_FLOAT32 ? 4 : 8;
+    const size_t pitch = k64 + 16, wave = 16 * pitch + 16 * kOutPitch + 64;
+    // Up to two workgroups of 16 rows x 64 channels a compute unit: 338 rows, 1024 -> 512 take 8 us so, 12 us by tiles;
+    // 1352 rows, with four rounds of workgroups, 18 and 12.
+    if ((rows + 15) / 16 * (n64 / 64) <= 512 && 16 * pitch + 64 <= 64 * 1024) {
+        p.how = ProductPlan::kFew;
+        p.lds = 16 * pitch + 64;
+        return p;
+    }
+    // Rows of up to 1024 bytes and weights that leave LDS room for eight wavefronts' rows; with longer rows (512 -> 128:
+    // 37 us by 16 rows, 31 by tiles) or with the weights in two halves the codes are better taken once, into memory.
+    p.lds = n64 * (pitch + 8) + kRowWaves * wave;
+    if (k64 <= 64 * V && p.lds <= 160 * 1024) {
+        p.how = ProductPlan::kRows;
+        p.lanes = std::max(4, pow2_at_least((k64 / V + 3) / 4));
+        return p;
+    }
+    p.how = ProductPlan::kTile;
+    return p;
+}
+
+template <class TX, class T, bool kWhole>
+void run_product(const ProductPlan &p, const TX *x, int64_t ldx, const float *xs, int64_t rows, int k, const int8_t *w, int64_t ldw, const float *ws,
+                 int n, const float *bias, T *y, int64_t ldy, int8_t *codes, int64_t ldc, float *scale, hipStream_t st)
+{
+    if (p.how == ProductPlan::kFew) {
+        k_int8_few<TX, T, kWhole><<<dim3((unsigned)((rows + 15) / 16), (n + 63) / 64), kThreads, p.lds, st>>>(x, ldx, xs, rows, k, w, ldw, ws, n, bias,
+                                                                                                              y, ldy, codes, ldc, scale);
+        return;
+    }
+    // as many workgroups as the compute units hold at once, or as there are rows for
+    const int64_t held = 256 * (int64_t)(160 * 1024 / p.lds), asked = (rows + 16 * kRowWaves - 1) / (16 * kRowWaves);
+    const unsigned blocks = (unsigned)std::min(held, asked);
+#define CALL(G) k_int8_rows<TX, T, G, kWhole><<<dim3(blocks), 64 * kRowWaves, p.lds, st>>>(x, ldx, xs, rows, k, p.lanes, w, ldw, ws, n, bias, y, ldy, codes, ldc, scale)
+    if (p.lanes <= 4) CALL(1);
+    else if (p.lanes <= 8) CALL(2);
+    else CALL(4);
+#undef CALL
+}
+
+}  // namespace
+
+bool product_needs_codes(int64_t rows, int32_t k, int32_t n, int32_t x_type)
+{
+    return x_type != YH_INT8 && plan_product(rows, k, n, x_type).how == ProductPlan::kTile;
+}
+
+hipError_t launch_int8_product(const Rows &x, const float *x_scale, int64_t rows, int32_t k,
+                               const int8_t *w, int64_t ldw, const float *w_scale, int32_t n, const float *bias,
+                               void *y, int64_t ldy, int32_t type, int8_t *codes, int64_t ldc, float *scale, hipStream_t st)
+{
+    const ProductPlan p = plan_product(rows, k, n, x.type);
+    if (p.how != ProductPlan::kTile) {
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            const auto go = [&](auto tx) {
+                using TX = decltype(tx);
+                // 16-byte vectors of weights and of x that end with the row, or any length
+                const auto call = k % 16 == 0 ? run_product<TX, T, true> : run_product<TX, T, false>;
+                call(p, static_cast<const TX *>(x.p), x.ld, x_scale, rows, k, w, ldw, w_scale, n, bias, static_cast<T *>(y), ldy, codes, ldc, scale, st);
+            };
+            if (x.type == YH_INT8) go((int8_t)0);
+            else with_type(x.type, go);
+        });
+        return hipGetLastError();
+    }
+    const int8_t *q = static_cast<const int8_t *>(x.p);
+    int64_t ldq = x.ld;
+    if (x.type != YH_INT8) {
+        const hipError_t e = launch_quantize(x, rows, k, codes, ldc, scale, st);
+        if (e != hipSuccess) return e;
+        q = codes, ldq = ldc, x_scale = scale;
+    }
     with_type(type, [&](auto t) {
         using T = decltype(t);
 #define CALL(BM, BN)                                                                                                        \
         do {                                                                                                                \
             const int tn = (n + BN - 1) / BN;                                                                               \
             k_int8_tile<T, BM, BN><<<dim3((unsigned)((rows + BM - 1) / BM * tn)), kThreads, 0, st>>>(                       \
-                x, ldx, x_scale, rows, k, w, ldw, w_scale, n, bias, static_cast<T *>(y), ldy, tn);                          \
+                q, ldq, x_scale, rows, k, w, ldw, w_scale, n, bias, static_cast<T *>(y), ldy, tn);                          \
         } while (0)
         // large tiles where they fill the card, small ones where there are few rows
         if ((rows + 127) / 128 * ((n + 127) / 128) >= 256) CALL(128, 128);
-        else CALL(32, 64);
+        else CALL(64, 64);
 #undef CALL
     });
     return hipGetLastError();

@@ -32,9 +32,11 @@ hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, cons
                                 const float *gamma, const float *invstd, float slope, void *dz, int64_t lddz,
                                 float *dgamma, float *dbeta, void *workspace, hipStream_t st);
 
-hipError_t launch_int8_product(const int8_t *x, int64_t ldx, const float *x_scale, int64_t rows, int32_t k,
+// codes, scale: where the codes of a float x are left; null if nobody wants them and product_needs_codes() says no.
+bool product_needs_codes(int64_t rows, int32_t k, int32_t n, int32_t x_type);
+hipError_t launch_int8_product(const Rows &x, const float *x_scale, int64_t rows, int32_t k,
                                const int8_t *w, int64_t ldw, const float *w_scale, int32_t n, const float *bias,
-                               void *y, int64_t ldy, int32_t type, hipStream_t st);
+                               void *y, int64_t ldy, int32_t type, int8_t *codes, int64_t ldc, float *scale, hipStream_t st);
 
 int weight_grad_chunks(int64_t rows, int32_t n, int32_t k);     // pieces the rows are cut into
 hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, const float *scale, int64_t rows,

@@ -98,7 +98,7 @@ int yh_matmul_int8_workspace_bytes(int64_t rows, int32_t k, int32_t n, int32_t x
     if (!bytes) return yh::report(YH_ERR_INVALID_ARG, "bytes is null");
     if (x_dtype != YH_INT8) YH_TRY(check_float_type(x_dtype, "x_dtype"));
     YH_TRY(check_sizes(rows, k, n));
-    *bytes = x_dtype == YH_INT8 || want_codes ? 0 : (size_t)rows * (codes_pitch(k) + 4);
+    *bytes = want_codes || !yh::product_needs_codes(rows, k, n, x_dtype) ? 0 : (size_t)rows * (codes_pitch(k) + 4);
     return YH_OK;
 }
 
@@ -127,21 +127,13 @@ int yh_matmul_int8(const void *x, int32_t x_dtype, int64_t ldx, const float *x_s
     if (rows == 0) return YH_OK;
     YH_TRY(yh::require_device());
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int8_t *q = static_cast<const int8_t *>(x);
-    const float *s = x_scale;
-    int64_t ldq = ldx;
-    if (!whole) {
-        if (!want) {
-            ldc = (int64_t)codes_pitch(k);
-            codes = static_cast<int8_t *>(workspace);
-            scale = reinterpret_cast<float *>(codes + rows * ldc);
-        }
-        YH_TRY(launched(yh::launch_quantize({x, ldx, x_dtype}, rows, k, codes, ldc, scale, st), "quantize launch"));
-        q = codes;
-        s = scale;
-        ldq = ldc;
+    if (!want && need) {
+        ldc = (int64_t)codes_pitch(k);
+        codes = static_cast<int8_t *>(workspace);
+        scale = reinterpret_cast<float *>(codes + rows * ldc);
     }
-    return launched(yh::launch_int8_product(q, ldq, s, rows, k, w, ldw, w_scale, n, bias, y, ldy, y_dtype, st), "product launch");
+    return launched(yh::launch_int8_product({x, ldx, x_dtype}, x_scale, rows, k, w, ldw, w_scale, n, bias, y, ldy, y_dtype, codes, ldc, scale, st),
+                    "product launch");
 }
 
 int yh_weight_grad_workspace_bytes(int64_t rows, int32_t n, int32_t k, size_t *bytes)
