@@ -135,7 +135,7 @@ def test_refusals_of_the_norm():
     _refused(f(r=0x1002), ali, 'residual')
     _refused(f(lda=7), inv, 'a: 7')
     _refused(f(ldk=7), inv, 'kept: 7')
-    _refused(f(size=8), wsp, 'workspace')
+    _refused(f(rows=100000, size=8), wsp, 'workspace')
 
     def b(da=OK[0], ld=8, t=F32, rows=4, c=8, kept=OK[1], ldk=8, s=OK[2], g=OK[3], i=OK[3], dz=OK[4], ldz=8, dg=OK[5], db=OK[5],
           work=OK[6], size=1 << 20):
@@ -146,7 +146,7 @@ def test_refusals_of_the_norm():
     _refused(b(s=None), inv, 'scale')
     _refused(b(dg=None), inv, 'dgamma')
     _refused(b(dz=0x5002), ali, 'dz')
-    _refused(b(work=None), wsp, 'workspace')
+    _refused(b(rows=100000, work=None), wsp, 'workspace')
 
 
 def test_workspace_sizes():
@@ -163,8 +163,8 @@ def test_workspace_sizes():
     # the pieces of the rows never take more than their number times the result, and that number is bounded
     for rows, a, b in ((1, 1, 1), (700000, 64, 128), (10816, 512, 1024), (50000, 1536, 1536)):
         assert ask(lib.yh_weight_grad_workspace_bytes, rows, a, b) <= 1024 * (a * b + a) * 4
-    assert ask(lib.yh_norm_act_workspace_bytes, 1, 1, F32) >= 16 + 12
-    assert ask(lib.yh_norm_act_workspace_bytes, 700000, 64, BF16) <= 64 * (1100 * 16 + 12)
+    assert ask(lib.yh_norm_act_workspace_bytes, 1, 1, F32) == 0                # few rows are summed by one workgroup a channel
+    assert 0 < ask(lib.yh_norm_act_workspace_bytes, 700000, 64, BF16) <= 64 * 1100 * 16
     assert lib.yh_norm_act_workspace_bytes(0, 8, F32, ctypes.byref(n)) == _abi.YH_ERR_INVALID_ARG
     for fn, a in ((lib.yh_matmul_int8_workspace_bytes, (1, 1, 1, 0, 0)), (lib.yh_weight_grad_workspace_bytes, (1, 1, 1)),
                   (lib.yh_norm_act_workspace_bytes, (1, 1, 0))):

@@ -221,19 +221,12 @@ struct NormStats {
     }
 };
 
-// What the elementwise pass of the backward takes from a channel's sums: coef = gamma * invstd, dbeta / M, dgamma / M.
 struct NormGrads {
-    int64_t rows;
-    int cols;
-    const float *gamma, *invstd;
-    float *dgamma, *dbeta, *coef;
+    float *dgamma, *dbeta;
     __device__ __forceinline__ void finish(int c, double b, double g) const
     {
         dbeta[c] = (float)b;
         dgamma[c] = (float)g;
-        coef[c] = gamma[c] * invstd[c];
-        coef[cols + c] = (float)(b / (double)rows);
-        coef[2 * (int64_t)cols + c] = (float)(g / (double)rows);
     }
 };
 
@@ -496,7 +489,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_finish(const double *par
 
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
-                                                              int64_t rows, int cols, float slope, const float *coef, T *dz, int64_t ldz, int lanes, int64_t waves)
+                                                              int64_t rows, int cols, float slope, const float *gamma, const float *invstd,
+                                                              const float *dgamma, const float *dbeta, T *dz, int64_t ldz, int lanes, int64_t waves)
 {
     constexpr int V = RowVec<T>::V;
     const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), rpw = 64 / lanes;
@@ -505,9 +499,17 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const int c = c0 + (i * lanes + sub) * V;
-        load_vec<float, V>(g[i], coef + c, cols - c);
-        load_vec<float, V>(cb[i], coef + cols + c, cols - c);
-        load_vec<float, V>(cg[i], coef + 2 * (int64_t)cols + c, cols - c);
+        float is[V];
+        load_vec<float, V>(g[i], gamma + c, cols - c);
+        load_vec<float, V>(is, invstd + c, cols - c);
+        load_vec<float, V>(cb[i], dbeta + c, cols - c);
+        load_vec<float, V>(cg[i], dgamma + c, cols - c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            g[i][j] *= is[j];
+            cb[i][j] = (float)((double)cb[i][j] / (double)rows);
+            cg[i][j] = (float)((double)cg[i][j] / (double)rows);
+        }
     }
     for (int64_t w0 = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); w0 * rpw < rows; w0 += waves) {
         const int64_t row = w0 * rpw + lane / lanes;
@@ -634,8 +636,7 @@ hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, cons
         using T = decltype(t);
         const T *p = static_cast<const T *>(da.p);
         const ReducePlan d = plan_reduce(rows, cols, RowVec<T>::V);
-        float *coef = reinterpret_cast<float *>(part + 2 * (int64_t)cols * d.blocks);
-        const NormGrads out{rows, cols, gamma, invstd, dgamma, dbeta, coef};
+        const NormGrads out{dgamma, dbeta};
         k_norm_grad_sums<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, da.ld, kept, ldk, scale, rows, cols, slope, d.tx, part, out);
         const int lanes = d.blocks > 64 ? kThreads : 64;
         if (d.blocks > 1)
@@ -644,7 +645,7 @@ hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, cons
         const int vecs = std::min(4, r.vecs), step = (vecs <= 1 ? 1 : vecs <= 2 ? 2 : 4) * r.lanes * RowVec<T>::V;
         const unsigned blocks = std::min(2048u, waves_to_blocks((rows * r.lanes + 63) / 64));
 #define CALL(IT) k_norm_grad_apply<T, IT><<<dim3(blocks, (cols + step - 1) / step), kThreads, 0, st>>>( \
-            p, da.ld, kept, ldk, scale, rows, cols, slope, coef, static_cast<T *>(dz), lddz, r.lanes, (int64_t)blocks * (kThreads / 64))
+            p, da.ld, kept, ldk, scale, rows, cols, slope, gamma, invstd, dgamma, dbeta, static_cast<T *>(dz), lddz, r.lanes, (int64_t)blocks * (kThreads / 64))
         if (vecs <= 1) CALL(1);
         else if (vecs <= 2) CALL(2);
         else CALL(4);

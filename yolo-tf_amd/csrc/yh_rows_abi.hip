@@ -184,7 +184,8 @@ int yh_norm_act_workspace_bytes(int64_t rows, int32_t c, int32_t dtype, size_t *
     YH_TRY(check_float_type(dtype, "dtype"));
     YH_TRY(check_sizes(rows, c, 1));
     if (rows < 1) return yh::report(YH_ERR_INVALID_ARG, "statistics of no rows");
-    *bytes = (size_t)c * (2 * sizeof(double) * yh::norm_blocks(rows, c, dtype) + 3 * sizeof(float));
+    const int blocks = yh::norm_blocks(rows, c, dtype);
+    *bytes = blocks > 1 ? (size_t)c * 2 * sizeof(double) * blocks : 0;
     return YH_OK;
 }
 

@@ -78,18 +78,18 @@ def _codes(q, dev, what):
     return _rows(q, what)
 
 
-def _new_codes(shape, dev):
-    """int8 codes of `shape` whose rows start at multiples of 16 bytes: a view of a wider buffer where needed."""
+def _new_codes(x, shape):
+    """int8 codes of x's `shape` whose rows start at multiples of 16 bytes: a view of a wider buffer where needed."""
     cols = shape[-1]
+    if cols % 16 == 0:
+        return x.new_empty(shape, dtype=torch.int8), cols
     wide = (cols + 15) // 16 * 16
-    if wide == cols:
-        return torch.empty(shape, dtype=torch.int8, device=dev), cols
-    return torch.empty(shape[:-1] + (wide,), dtype=torch.int8, device=dev)[..., :cols], wide
+    return x.new_empty(shape[:-1] + (wide,), dtype=torch.int8)[..., :cols], wide
 
 
 def _call(dev, fn, *args):
     """One library call on `dev`'s current stream."""
-    if torch.cuda.current_device() == dev.index:
+    if torch._C._cuda_getDevice() == dev.index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
@@ -98,8 +98,8 @@ def _call(dev, fn, *args):
         _abi.check(rc)
 
 
-def _scratch(fn_name, dev, *sizes):
-    """(pointer, bytes, tensor that keeps it) of a workspace for one call."""
+def _scratch(fn_name, owner, *sizes):
+    """(pointer, bytes, tensor that keeps it) of a workspace for one call, on the device of the tensor `owner`."""
     n = _sizes.get((fn_name, sizes))
     if n is None:
         out = ctypes.c_size_t(0)
@@ -109,7 +109,7 @@ def _scratch(fn_name, dev, *sizes):
         n = _sizes[(fn_name, sizes)] = out.value
     if n == 0:
         return None, 0, None
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    ws = owner.new_empty(n, dtype=torch.uint8)
     return ws.data_ptr(), n, ws
 
 
@@ -121,8 +121,8 @@ def quantize_rows(x):
     kind = _float_type(x.dtype, 'x')
     xr, rows, cols, ld = _rows(x, 'x')
     shape = tuple(x.shape)
-    codes, ldc = _new_codes(shape, dev)
-    scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    codes, ldc = _new_codes(x, shape)
+    scale = x.new_empty(shape[:-1], dtype=torch.float32)
     _call(dev, _abi.load().yh_quantize_rows, xr.data_ptr(), kind, ld, rows, cols, codes.data_ptr(), ldc, scale.data_ptr())
     return codes, scale
 
@@ -133,7 +133,7 @@ def dequantize_rows(codes, scale, dtype=torch.float32):
     kind = _float_type(dtype, 'dtype')
     qr, rows, cols, ld = _codes(codes, dev, 'codes')
     scale = _vector(scale, rows, dev, 'scale')
-    x = torch.empty(codes.shape, dtype=dtype, device=dev)
+    x = codes.new_empty(codes.shape, dtype=dtype)
     _call(dev, _abi.load().yh_dequantize_rows, qr.data_ptr(), ld, scale.data_ptr(), rows, cols, x.data_ptr(), kind, cols)
     return x
 
@@ -167,13 +167,13 @@ def matmul_int8(x, w_codes, w_scale, bias=None, x_scale=None, out_dtype=None, wa
         out_dtype = x.dtype if out_dtype is None else out_dtype
     out_kind = _float_type(out_dtype, 'out_dtype')
     shape = tuple(x.shape)
-    y = torch.empty(shape[:-1] + (n,), dtype=out_dtype, device=dev)
+    y = x.new_empty(shape[:-1] + (n,), dtype=out_dtype)
     codes = scale = None
     ldc = 0
     if want_codes:
-        codes, ldc = _new_codes(shape, dev)
-        scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
-    ws, nbytes, keep = _scratch('yh_matmul_int8_workspace_bytes', dev, rows, k, n, kind, 1 if want_codes else 0)
+        codes, ldc = _new_codes(x, shape)
+        scale = x.new_empty(shape[:-1], dtype=torch.float32)
+    ws, nbytes, keep = _scratch('yh_matmul_int8_workspace_bytes', x, rows, k, n, kind, 1 if want_codes else 0)
     _call(dev, lib.yh_matmul_int8, xr.data_ptr(), kind, ldx, x_scale.data_ptr() if whole else None, rows, k,
           wr.data_ptr(), ldw, w_scale.data_ptr(), n, None if bias is None else bias.data_ptr(), y.data_ptr(), out_kind, n,
           codes.data_ptr() if want_codes else None, ldc, scale.data_ptr() if want_codes else None, ws, nbytes)
@@ -190,9 +190,9 @@ def weight_grad(dy, codes, scale, want_bias=False):
     if qrows != rows:
         raise ValueError('dy has %d rows, codes %d' % (rows, qrows))
     scale = _vector(scale, rows, dev, 'scale')
-    dw = torch.empty((n, k), dtype=torch.float32, device=dev)
-    db = torch.empty((n,), dtype=torch.float32, device=dev) if want_bias else None
-    ws, nbytes, keep = _scratch('yh_weight_grad_workspace_bytes', dev, rows, n, k)
+    dw = dy.new_empty((n, k), dtype=torch.float32)
+    db = dy.new_empty((n,), dtype=torch.float32) if want_bias else None
+    ws, nbytes, keep = _scratch('yh_weight_grad_workspace_bytes', dy, rows, n, k)
     _call(dev, _abi.load().yh_weight_grad, dr.data_ptr(), kind, ldd, qr.data_ptr(), ldq, scale.data_ptr(), rows, n, k,
           dw.data_ptr(), db.data_ptr() if want_bias else None, ws, nbytes)
     return (dw, db) if want_bias else dw
@@ -207,7 +207,7 @@ def input_grad(dy, w_codes, w_scale):
     if w_codes.dim() != 2 or wn != n:
         raise ValueError('w_codes must be [%d, K], got %s' % (n, tuple(w_codes.shape)))
     w_scale = _vector(w_scale, n, dev, 'w_scale')
-    dx = torch.empty(tuple(dy.shape[:-1]) + (k,), dtype=dy.dtype, device=dev)
+    dx = dy.new_empty(tuple(dy.shape[:-1]) + (k,))
     _call(dev, _abi.load().yh_input_grad, dr.data_ptr(), kind, ldd, wr.data_ptr(), ldw, w_scale.data_ptr(), rows, n, k,
           dx.data_ptr(), k)
     return dx
@@ -270,12 +270,12 @@ def norm_act(z, gamma, beta, eps, slope, residual=None, running=None, momentum=0
             if _vector(t, c, dev, 'running').data_ptr() != t.data_ptr():
                 raise ValueError('the running statistics must be contiguous: they are updated in place')
     shape, slope = tuple(z.shape), float(slope)
-    a = torch.empty(shape, dtype=z.dtype, device=dev)
+    a = z.new_empty(shape)
     pitch = (c + 15) // 16 * 16 if want_kept else 0
     head = rows * (pitch + 4) if want_kept else 0
-    store = torch.empty(head + 8 * c, dtype=torch.uint8, device=dev)
+    store = z.new_empty(head + 8 * c, dtype=torch.uint8)
     at = store.data_ptr()
-    ws, nbytes, keep = _scratch('yh_norm_act_workspace_bytes', dev, rows, c, kind)
+    ws, nbytes, keep = _scratch('yh_norm_act_workspace_bytes', z, rows, c, kind)
     _call(dev, _abi.load().yh_norm_act_forward, zr.data_ptr(), ldz, None if rr is None else rr.data_ptr(), ldr, kind, rows, c,
           gamma.data_ptr(), beta.data_ptr(), float(eps), slope, a.data_ptr(), c,
           at if want_kept else None, pitch, at + rows * pitch if want_kept else None, at + head, at + head + 4 * c,
@@ -293,12 +293,11 @@ def norm_act_backward(da, kept):
         raise ValueError('da must be shaped like the forward call\'s z, %s, on %s; got %s' % (kept.shape, kept.store.device, tuple(da.shape)))
     dr, rows, c, ldd = _rows(da, 'da')
     gamma = _vector(kept.gamma, c, dev, 'gamma')
-    dz = torch.empty(kept.shape, dtype=da.dtype, device=dev)
-    dgamma = torch.empty(c, dtype=torch.float32, device=dev)
-    dbeta = torch.empty(c, dtype=torch.float32, device=dev)
+    dz = da.new_empty(kept.shape)
+    dgamma, dbeta = da.new_empty(c, dtype=torch.float32), da.new_empty(c, dtype=torch.float32)
     at = kept.store.data_ptr()
     scale = at + rows * kept.pitch
-    ws, nbytes, keep = _scratch('yh_norm_act_workspace_bytes', dev, rows, c, kind)
+    ws, nbytes, keep = _scratch('yh_norm_act_workspace_bytes', da, rows, c, kind)
     _call(dev, _abi.load().yh_norm_act_backward, dr.data_ptr(), ldd, kind, rows, c, at, kept.pitch, scale,
           gamma.data_ptr(), scale + 4 * rows + 4 * c, kept.slope, dz.data_ptr(), c, dgamma.data_ptr(), dbeta.data_ptr(), ws, nbytes)
     return dz, dgamma, dbeta
