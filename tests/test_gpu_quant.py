@@ -310,9 +310,9 @@ def test_norm_backward(gpu, m, c, dtype):
     g = qc.f64(gamma) * qc.f64(kept.invstd)
     cb, cg = du.sum(0) / m, (du * xq).sum(0) / m
     want = g * (du - cb - xq * cg)
-    # on any of the three terms: the sum rounded, divided, two subtractions, g (a product) and the product with it, six
-    # half steps in all
-    bound = np.abs(g) * 6.01 * qc.U * (np.abs(du) + np.abs(cb) + np.abs(xq * cg)) + qc.HALF_STEP[dtype] * 1.01 * np.abs(want) + qc.TINY[dtype] + 1e-40
+    # on any of the three terms: the sum rounded, times 1 / M (two more), two subtractions, g (a product) and the product
+    # with it, seven half steps in all; the third term has one more, from the product with xq
+    bound = np.abs(g) * 8.01 * qc.U * (np.abs(du) + np.abs(cb) + np.abs(xq * cg)) + qc.HALF_STEP[dtype] * 1.01 * np.abs(want) + qc.TINY[dtype] + 1e-40
     assert dz.dtype == dtype and (np.abs(qc.f64(dz) - want) <= bound).all()
 
 

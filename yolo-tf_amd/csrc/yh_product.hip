@@ -481,29 +481,29 @@ __global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx,
     v4i a[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) a[i] = load_elements<int8_t, kWhole>(wr + i * 64 + quad * 16, k - i * 64 - quad * 16);
+    const int64_t row = first + r16;
+    const int c = n0 + quad * 4;
+    float sc[4], bi[4] = {0.0f, 0.0f, 0.0f, 0.0f}, o[4];
+    load_vec<float, 4>(sc, ws + c, n - c);
+    if (bias) load_vec<float, 4>(bi, bias + c, n - c);
     if (blockIdx.y) codes = nullptr, scale = nullptr;
     if constexpr (sizeof(TX) == 1) code_rows_given<kWhole>(x, ldx, xs, first, rows, k, k64, lx, ls);
     else code_four_rows<TX, kWhole>(x, ldx, xs, first, rows, k, k64, lx, ls, codes, ldc, scale);
     __syncthreads();
-    v4i acc = {0, 0, 0, 0};
+    v4i acc = {0, 0, 0, 0}, odd = {0, 0, 0, 0};            // two chains of sums: one would wait for itself
     const int8_t *at = lx + r16 * pitch + quad * 16;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
+    for (int i = 0; i < kAhead; i += 2) {
         if (i * 64 < k64) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], *reinterpret_cast<const v4i *>(at + i * 64), acc, 0, 0, 0);
+        if (i * 64 + 64 < k64) odd = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i + 1], *reinterpret_cast<const v4i *>(at + i * 64 + 64), odd, 0, 0, 0);
+    }
+    acc += odd;
     for (int q = kAhead * 64; q < k64; q += 64)
         acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_elements<int8_t, kWhole>(wr + q + quad * 16, k - q - quad * 16), *reinterpret_cast<const v4i *>(at + q), acc, 0, 0, 0);
-    const int64_t row = first + r16;
-    const int c = n0 + quad * 4;
     if (row >= rows) return;
     const float s = ls[r16];
-    float sc[4], bi[4], o[4];
-    load_vec<float, 4>(sc, ws + c, n - c);
-    if (bias) load_vec<float, 4>(bi, bias + c, n - c);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        o[e] = (float)acc[e] * s * sc[e];
-        if (bias) o[e] += bi[e];
-    }
+    for (int e = 0; e < 4; ++e) o[e] = (float)acc[e] * s * sc[e] + bi[e];
     store_vec<T, 4>(y + row * ldy + c, o, n - c);
 }
 

@@ -130,12 +130,25 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
     return lo | hi;
 }
 
-// Largest |value| bits of a row, over the `lanes` (a power of two) neighbouring lanes that hold it.  Magnitudes are
-// compared as integers: every NaN is above infinity, infinity above every number.
+// f over the `lanes` (a power of two) neighbouring lanes of a group, the result in all of them; the whole wavefront takes
+// part.  Up to 16 lanes by data-parallel moves inside the vector unit, beyond by LDS permutes.
+template <class F>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t m, int lanes, F f)
+{
+    if (lanes > 1) m = f(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, true));    // lane ^ 1
+    if (lanes > 2) m = f(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));    // lane ^ 2
+    if (lanes > 4) m = f(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, true));   // mirrored in eight
+    if (lanes > 8) m = f(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xf, 0xf, true));   // mirrored in sixteen
+    if (lanes > 16) m = f(m, (uint32_t)__shfl_xor((int)m, 16));
+    if (lanes > 32) m = f(m, (uint32_t)__shfl_xor((int)m, 32));
+    return m;
+}
+
+// Largest |value| bits of a row.  Magnitudes are compared as integers: every NaN is above infinity, infinity above every
+// number.
 __device__ __forceinline__ uint32_t row_max(uint32_t m, int lanes)
 {
-    for (int o = 1; o < lanes; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-    return m;
+    return over_lanes(m, lanes, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
 struct RowScale { float r, s; bool live; };

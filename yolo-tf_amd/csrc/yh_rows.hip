@@ -19,11 +19,13 @@ int pow2_at_least(int v)
 // `lanes` vectors apart.  Four vectors a lane keep 4 KiB of loads in flight a wavefront; rows shorter than that share
 // the wavefront, with at least eight lanes (128 contiguous bytes) each.
 struct RowPlan { int lanes, vecs; };
-RowPlan plan_row(int cols, int V)
+RowPlan plan_row(int64_t rows, int cols, int V)
 {
     const int nv = (cols + V - 1) / V;
     RowPlan p;
     p.lanes = std::min(64, std::max(std::min(8, pow2_at_least(nv)), pow2_at_least((nv + 3) / 4)));
+    // few rows leave most of the card idle: as many lanes a row as there are vectors
+    if (rows * p.lanes < 64 * 1024) p.lanes = std::min(64, pow2_at_least(nv));
     p.vecs = (nv + p.lanes - 1) / p.lanes;
     return p;
 }
@@ -174,42 +176,52 @@ ReducePlan plan_reduce(int64_t rows, int cols, int V)
     return p;
 }
 
-// Adds the threads' pairs over ty, into those with ty == 0, and writes the workgroup's pair of each channel to
-// part[2][cols][blocks] where there is more than one workgroup.
-template <int V>
-__device__ __forceinline__ void reduce_pairs(double (&s1)[V], double (&s2)[V], int tx, int ty, int TX, int cvec, int cols, double *part, int blocks)
+// Adds the threads' pairs over ty: first over the lanes of a wavefront that hold the same channels, then over the four
+// wavefronts through LDS, a thread a channel.  Where there is more than one workgroup its pair goes to
+// part[2][cols][blocks], otherwise to out.finish(channel, sum, sum).
+template <int V, class Out>
+__device__ __forceinline__ void reduce_pairs(double (&s1)[V], double (&s2)[V], int TX, int cols, double *part, const Out &out)
 {
-    __shared__ double buf[kThreads * V];
+    constexpr int W = kThreads / 64;
+    __shared__ double buf[2 * V][W][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int o = TX; o < 64; o <<= 1)
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        double (&s)[V] = which ? s2 : s1;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < V; ++j) buf[j * kThreads + threadIdx.x] = s[j];
-        for (int half = kThreads / 2; half >= TX; half >>= 1) {
-            __syncthreads();
-            if ((int)threadIdx.x < half)
-#pragma unroll
-                for (int j = 0; j < V; ++j) buf[j * kThreads + threadIdx.x] += buf[j * kThreads + threadIdx.x + half];
+        for (int j = 0; j < V; ++j) {
+            s1[j] += __shfl_xor(s1[j], o);
+            s2[j] += __shfl_xor(s2[j], o);
         }
-        if (ty == 0)
+    if (lane < TX)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const int c = cvec * V + j;
-                s[j] = buf[j * kThreads + tx];
-                if (blocks > 1 && c < cols) part[((int64_t)which * cols + c) * blocks + blockIdx.x] = s[j];
-            }
+        for (int j = 0; j < V; ++j) {
+            buf[2 * j][wave][lane] = s1[j];
+            buf[2 * j + 1][wave][lane] = s2[j];
+        }
+    __syncthreads();
+    for (int t = threadIdx.x; t < TX * V; t += kThreads) {
+        const int c = blockIdx.y * TX * V + t, x = t / V, j = t % V;
+        if (c >= cols) continue;
+        const double a = (buf[2 * j][0][x] + buf[2 * j][1][x]) + (buf[2 * j][2][x] + buf[2 * j][3][x]);
+        const double b = (buf[2 * j + 1][0][x] + buf[2 * j + 1][1][x]) + (buf[2 * j + 1][2][x] + buf[2 * j + 1][3][x]);
+        if (gridDim.x > 1) {
+            part[(int64_t)c * gridDim.x + blockIdx.x] = a;
+            part[((int64_t)cols + c) * gridDim.x + blockIdx.x] = b;
+        } else {
+            out.finish(c, a, b);
+        }
     }
 }
 
 // What follows from a channel's sums of (z - first) and of its square.
+template <class T>
 struct NormStats {
+    const T *first;                                      // z's first row
     int64_t rows;
     double eps, momentum;
     float *mean, *invstd, *running_mean, *running_var;
-    __device__ __forceinline__ void finish(int c, float first, double s1, double s2) const
+    __device__ __forceinline__ void finish(int c, double s1, double s2) const
     {
-        const double m = (double)rows, d = s1 / m, mu = (double)first + d;
+        const double m = (double)rows, d = s1 / m, mu = (double)(float)first[c] + d;
         double var = s2 / m - d * d;
         if (var < 0.0) var = 0.0;                        // a NaN stays one
         mean[c] = (float)mu;
@@ -232,7 +244,7 @@ struct NormGrads {
 
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int TX, double *part,
-                                                         NormStats out)
+                                                         NormStats<T> out)
 {
     constexpr int V = RowVec<T>::V, U = 4;
     const int tx = threadIdx.x & (TX - 1), ty = threadIdx.x / TX, TY = kThreads / TX;
@@ -261,17 +273,15 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t row
 #pragma unroll
             for (int i = 0; i < U; ++i) add(v[i]);
         }
-    for (; r < rows; r += step)
-        for (int i = 0; i < U && r + i * TY < rows; ++i) {
-            float v[V];
-            load_vec<T, V>(v, p + (r + i * TY) * ldz, left);
-            add(v);
-        }
-    reduce_pairs<V>(s1, s2, tx, ty, TX, cvec, cols, part, gridDim.x);
-    if (gridDim.x == 1 && ty == 0)
+    for (; r < rows; r += step) {                    // rows past the end are read as the last one and left out
+        float v[U][V];
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < left) out.finish(c + j, first[j], s1[j], s2[j]);
+        for (int i = 0; i < U; ++i) load_vec<T, V>(v[i], p + min(r + i * TY, rows - 1) * ldz, left);
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (r + i * TY < rows) add(v[i]);
+    }
+    reduce_pairs<V>(s1, s2, TX, cols, part, out);
 }
 
 // A channel's pair of sums over its partials, by `lanes` threads (64: a wavefront, or 256: the workgroup; few partials
@@ -303,12 +313,12 @@ __device__ __forceinline__ void sum_partials(const double *p, const double *q, i
 }
 
 template <class T>
-__global__ __launch_bounds__(kThreads) void k_norm_stats_finish(const double *part, int blocks, const T *z, int cols, int lanes, NormStats out)
+__global__ __launch_bounds__(kThreads) void k_norm_stats_finish(const double *part, int blocks, int cols, int lanes, NormStats<T> out)
 {
     const int per = kThreads / lanes, c = min((int)blockIdx.x * per + (int)threadIdx.x / lanes, cols - 1), at = threadIdx.x & (lanes - 1);
     double s1, s2;
     sum_partials(part + (int64_t)c * blocks, part + ((int64_t)cols + c) * blocks, blocks, at, lanes, s1, s2);
-    if (at == 0 && (int)blockIdx.x * per + (int)threadIdx.x / lanes < cols) out.finish(c, (float)z[c], s1, s2);
+    if (at == 0 && (int)blockIdx.x * per + (int)threadIdx.x / lanes < cols) out.finish(c, s1, s2);
 }
 
 template <class T, int IT>
@@ -463,20 +473,21 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_
 #pragma unroll
             for (int i = 0; i < U; ++i) add(v[i], w[i], s[i]);
         }
-    for (; r < rows; r += step)
-        for (int i = 0; i < U && r + i * TY < rows; ++i) {
-            const int64_t rr = r + i * TY;
-            float v[V];
-            uint32_t w[V / 4];
-            load_vec<T, V>(v, da + rr * ldd + c, left);
-            load_bytes<V>(w, kept + rr * ldk + c, left);
-            add(v, w, scale[rr]);
-        }
-    reduce_pairs<V>(s1, s2, tx, ty, TX, cvec, cols, part, gridDim.x);
-    if (gridDim.x == 1 && ty == 0)
+    for (; r < rows; r += step) {
+        float v[U][V], s[U];
+        uint32_t w[U][V / 4];
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < left) out.finish(c + j, s1[j], s2[j]);
+        for (int i = 0; i < U; ++i) {
+            const int64_t rr = min(r + i * TY, rows - 1);
+            load_vec<T, V>(v[i], da + rr * ldd + c, left);
+            load_bytes<V>(w[i], kept + rr * ldk + c, left);
+            s[i] = scale[rr];
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (r + i * TY < rows) add(v[i], w[i], s[i]);
+    }
+    reduce_pairs<V>(s1, s2, TX, cols, part, out);
 }
 
 __global__ __launch_bounds__(kThreads) void k_norm_grad_finish(const double *part, int blocks, int cols, int lanes, NormGrads out)
@@ -495,6 +506,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64
     constexpr int V = RowVec<T>::V;
     const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), rpw = 64 / lanes;
     const int c0 = blockIdx.y * IT * lanes * V;
+    const float per_row = 1.0f / (float)rows;
     float g[IT][V], cb[IT][V], cg[IT][V];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
@@ -507,8 +519,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             g[i][j] *= is[j];
-            cb[i][j] = (float)((double)cb[i][j] / (double)rows);
-            cg[i][j] = (float)((double)cg[i][j] / (double)rows);
+            cb[i][j] *= per_row;
+            cg[i][j] *= per_row;
         }
     }
     for (int64_t w0 = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); w0 * rpw < rows; w0 += waves) {
@@ -565,7 +577,7 @@ hipError_t launch_quantize(const Rows &x, int64_t rows, int32_t cols, int8_t *co
     with_type(x.type, [&](auto t) {
         using T = decltype(t);
         const T *p = static_cast<const T *>(x.p);
-        const RowPlan r = plan_row(cols, RowVec<T>::V);
+        const RowPlan r = plan_row(rows, cols, RowVec<T>::V);
         if (r.vecs > 6) {
             k_quantize_long<T><<<dim3(row_blocks(rows)), kThreads, 0, st>>>(p, rows, cols, x.ld, codes, ldc, scale);
             return;
@@ -583,7 +595,7 @@ hipError_t launch_dequantize(const int8_t *codes, int64_t ldc, const float *scal
 {
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        const RowPlan r = plan_row(cols, RowVec<T>::V);
+        const RowPlan r = plan_row(rows, cols, RowVec<T>::V);
         const unsigned blocks = waves_to_blocks((rows * r.lanes + 63) / 64);
 #define CALL(IT) k_dequantize<T, IT><<<dim3(blocks), kThreads, 0, st>>>(codes, ldc, scale, rows, cols, static_cast<T *>(out), ldo, r.lanes)
         YH_WITH_VECS(r.vecs, CALL);
@@ -607,12 +619,12 @@ hipError_t launch_norm_forward(const Rows &z, const Rows &res, int64_t rows, int
         using T = decltype(t);
         const T *p = static_cast<const T *>(z.p), *q = static_cast<const T *>(res.p);
         const ReducePlan d = plan_reduce(rows, cols, RowVec<T>::V);
-        const NormStats out{rows, eps, momentum, mean, invstd, running_mean, running_var};
+        const NormStats<T> out{p, rows, eps, momentum, mean, invstd, running_mean, running_var};
         k_norm_stats<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, rows, cols, z.ld, d.tx, part, out);
         const int lanes = d.blocks > 64 ? kThreads : 64;
         if (d.blocks > 1)
-            k_norm_stats_finish<T><<<dim3((cols * lanes + kThreads - 1) / kThreads), kThreads, 0, st>>>(part, d.blocks, p, cols, lanes, out);
-        const RowPlan r = plan_row(cols, RowVec<T>::V);
+            k_norm_stats_finish<T><<<dim3((cols * lanes + kThreads - 1) / kThreads), kThreads, 0, st>>>(part, d.blocks, cols, lanes, out);
+        const RowPlan r = plan_row(rows, cols, RowVec<T>::V);
         if (r.vecs > 6) {
             k_norm_apply_long<T><<<dim3(row_blocks(rows)), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope,
                                                                             static_cast<T *>(a), lda, kept, ldk, scale);
@@ -641,7 +653,7 @@ hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, cons
         const int lanes = d.blocks > 64 ? kThreads : 64;
         if (d.blocks > 1)
             k_norm_grad_finish<<<dim3((cols * lanes + kThreads - 1) / kThreads), kThreads, 0, st>>>(part, d.blocks, cols, lanes, out);
-        const RowPlan r = plan_row(cols, RowVec<T>::V);
+        const RowPlan r = plan_row(rows, cols, RowVec<T>::V);
         const int vecs = std::min(4, r.vecs), step = (vecs <= 1 ? 1 : vecs <= 2 ? 2 : 4) * r.lanes * RowVec<T>::V;
         const unsigned blocks = std::min(2048u, waves_to_blocks((rows * r.lanes + 63) / 64));
 #define CALL(IT) k_norm_grad_apply<T, IT><<<dim3(blocks, (cols + step - 1) / step), kThreads, 0, st>>>( \
