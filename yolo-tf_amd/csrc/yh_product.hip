@@ -475,12 +475,14 @@ __global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx,
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, quad = lane >> 4;
     const int64_t first = (int64_t)blockIdx.x * 16;
     const int n0 = blockIdx.y * 64 + wave * 16;
-    int8_t *lx = lds;
-    float *ls = reinterpret_cast<float *>(lds + 16 * pitch);
-    const int8_t *wr = w + (int64_t)min(n0 + r16, n - 1) * ldw;
+    int8_t *turn = lds + wave * 4096, *lx = lds + 4 * 4096;      // a wavefront's weights on their way to its operands: 4 steps
+    float *ls = reinterpret_cast<float *>(lx + 16 * pitch);
+    // four lanes take a row's 64 bytes of a step
+    const int8_t *wr = w + (int64_t)min(n0 + (lane >> 2), n - 1) * ldw;
+    const int part = (lane & 3) * 16;
     v4i a[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) a[i] = load_elements<int8_t, kWhole>(wr + i * 64 + quad * 16, k - i * 64 - quad * 16);
+    for (int i = 0; i < kAhead; ++i) a[i] = load_elements<int8_t, kWhole>(wr + i * 64 + part, k - i * 64 - part);
     const int64_t row = first + r16;
     const int c = n0 + quad * 4;
     float sc[4], bi[4] = {0.0f, 0.0f, 0.0f, 0.0f}, o[4];
@@ -492,14 +494,28 @@ __global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx,
     __syncthreads();
     v4i acc = {0, 0, 0, 0}, odd = {0, 0, 0, 0};            // two chains of sums: one would wait for itself
     const int8_t *at = lx + r16 * pitch + quad * 16;
+    const auto four_steps = [&](const v4i *wv, int q) {
+        wave_sync();
 #pragma unroll
-    for (int i = 0; i < kAhead; i += 2) {
-        if (i * 64 < k64) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], *reinterpret_cast<const v4i *>(at + i * 64), acc, 0, 0, 0);
-        if (i * 64 + 64 < k64) odd = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i + 1], *reinterpret_cast<const v4i *>(at + i * 64 + 64), odd, 0, 0, 0);
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<v4i *>(turn + i * 1024 + chunk_at(lane >> 2, lane & 3)) = wv[i];
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (q + i * 64 >= k64) break;
+            v4i &sum = i & 1 ? odd : acc;
+            sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i *>(turn + i * 1024 + chunk_at(r16, quad)),
+                                                        *reinterpret_cast<const v4i *>(at + q + i * 64), sum, 0, 0, 0);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; i += 4)
+        if (i * 64 < k64) four_steps(a + i, i * 64);
+    for (int q = kAhead * 64; q < k64; q += 256) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = load_elements<int8_t, kWhole>(wr + q + i * 64 + part, k - q - i * 64 - part);
+        four_steps(a, q);
     }
     acc += odd;
-    for (int q = kAhead * 64; q < k64; q += 64)
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_elements<int8_t, kWhole>(wr + q + quad * 16, k - q - quad * 16), *reinterpret_cast<const v4i *>(at + q), acc, 0, 0, 0);
     if (row >= rows) return;
     const float s = ls[r16];
 #pragma unroll
@@ -931,7 +947,7 @@ ProductPlan plan_product(int64_t rows, int k, int n, int x_type)
     // 1352 rows, with four rounds of workgroups, 18 and 12.
     if ((rows + 15) / 16 * (n64 / 64) <= 512 && 16 * pitch + 64 <= 64 * 1024) {
         p.how = ProductPlan::kFew;
-        p.lds = 16 * pitch + 64;
+        p.lds = 4 * 4096 + 16 * pitch + 64;
         return p;
     }
     // Rows of up to 1024 bytes and weights that leave LDS room for eight wavefronts' rows; with longer rows (512 -> 128:
