@@ -201,6 +201,28 @@ def test_a_step_with_checkpoints_holds_less_memory(gpu):
     assert held['int8'] < held['float32'] / 2
 
 
+def test_a_step_under_autocast(gpu):
+    """The convolutions in bfloat16, the checkpoints beside them: gradients of the parameters' own type, near the plain
+    stack's under the same autocast."""
+    torch.manual_seed(9)
+    grads = {}
+    x = torch.randn(2, 32, 12, 12, device=gpu).contiguous(memory_format=torch.channels_last)
+    da = torch.randn(2, 48, 12, 12, device=gpu)
+    for mode in ('float32', 'int8'):
+        for kernel in (1, 3):
+            torch.manual_seed(9)
+            layer = _layer(32, 48, kernel, 1, True, 'float32', mode, gpu)
+            with torch.autocast('cuda', dtype=torch.bfloat16):
+                out = layer(x)
+            (out.float() * da).sum().backward()
+            grads[mode, kernel] = layer.conv.weight.grad
+            assert layer.conv.weight.grad.dtype == torch.float32 and torch.isfinite(layer.conv.weight.grad).all()
+    for kernel in (1, 3):
+        a, b = grads['int8', kernel], grads['float32', kernel]
+        # bfloat16 convolutions (2^-8 a term) and codes (2^-8 of a row's largest) on both sides of sums over 288 pixels
+        assert float((a - b).norm() / b.norm()) < 0.05
+
+
 def test_options_are_checked():
     with pytest.raises(ValueError, match='pointwise'):
         bb.Darknet19Head(2, 1, pointwise='int4')

@@ -13,7 +13,8 @@ is no CPU path: without a HIP device these functions raise.
 The functions of the first half compute; the second half binds them to autograd, for
 backbone.ConvBN (`pointwise='int8'`, `checkpoints='int8'`).  Their gradients take
 the roundings for the identity (straight through) and cannot be differentiated
-again."""
+again.  As with every autograd function, a backward pass is captured into a graph
+only while no eager graph of the same parameters is alive."""
 import ctypes
 
 import torch
@@ -308,11 +309,12 @@ class _LinearInt8(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, keep):
         w_codes, w_scale = quantize_rows(weight)
+        ctx.types = weight.dtype, None if bias is None else bias.dtype
+        bias = None if bias is None else bias.float()
         if not keep:
             return matmul_int8(x, w_codes, w_scale, bias)
         y, codes, scale = matmul_int8(x, w_codes, w_scale, bias, want_codes=True)
         ctx.save_for_backward(codes, scale, w_codes, w_scale)
-        ctx.types = weight.dtype, None if bias is None else bias.dtype
         return y
 
     @staticmethod
@@ -352,20 +354,22 @@ class _ConvKept(Function):
         codes, scale, weight = ctx.saved_tensors
         n, k = weight.shape[:2]
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        own = weight.to(dy.dtype)                           # under autocast the convolution ran in dy's type
+        dx = dw = db = None
         if weight.shape[2:] == (1, 1) and ctx.stride == 1:
             rows = dy.permute(0, 2, 3, 1)
-            dx = dw = db = None
             if need_x:
-                dx = (rows.reshape(-1, n) @ weight.reshape(n, k)).view(codes.shape).permute(0, 3, 1, 2)
+                dx = (rows.reshape(-1, n) @ own.reshape(n, k)).view(codes.shape).permute(0, 3, 1, 2)
             if need_w or need_b:
                 dw, db = weight_grad(rows, codes, scale, want_bias=True)
-                dw, db = dw.to(weight.dtype).view(weight.shape), db.to(weight.dtype)
-            return dx, dw, db if ctx.has_bias else None, None
-        x = dequantize_rows(codes, scale, ctx.dtype).permute(0, 3, 1, 2)
-        s = [ctx.stride, ctx.stride]
-        dx, dw, db = torch.ops.aten.convolution_backward(dy.contiguous(memory_format=torch.channels_last), x, weight, [n] if ctx.has_bias else None,
-                                                         s, [0, 0], [1, 1], False, [0, 0], 1, [need_x, need_w, need_b and ctx.has_bias])
-        return dx, dw, db, None
+                dw = dw.view(weight.shape)
+        else:
+            x = dequantize_rows(codes, scale, dy.dtype).permute(0, 3, 1, 2)
+            s = [ctx.stride, ctx.stride]
+            dx, dw, db = torch.ops.aten.convolution_backward(dy.contiguous(memory_format=torch.channels_last), x, own, [n] if ctx.has_bias else None,
+                                                             s, [0, 0], [1, 1], False, [0, 0], 1, [need_x, need_w, need_b and ctx.has_bias])
+        return (dx.to(ctx.dtype) if need_x else None, dw.to(weight.dtype) if need_w else None,
+                db.to(weight.dtype) if need_b and ctx.has_bias else None, None)
 
 
 def conv_kept(x, weight, bias, stride):
