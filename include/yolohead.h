@@ -457,7 +457,8 @@ int yh_input_grad(const void *dy, int32_t dtype, int64_t lddy, const int8_t *w, 
  *   running_* [c]: (1 - momentum) * running + momentum * (mean, var * rows / (rows - 1));
  *   mean, invstd [c]: outputs, invstd is read by the backward pass;
  *   rows >= 1 (one row: var is 0).  The statistics of a channel that holds an
- *   infinity or a NaN are NaN, and with them everything but the other channels' a.
+ *   infinity or a NaN are NaN, and with them everything but the other channels' a
+ *   and dbeta (a row's scale is one number for all its channels).
  * a may be residual, dz may be da (the same rows in place). */
 int yh_norm_act_workspace_bytes(int64_t rows, int32_t c, int32_t dtype, size_t *bytes);
 int yh_norm_act_forward(const void *z, int64_t ldz, const void *residual, int64_t ldr, int32_t dtype, int64_t rows, int32_t c,

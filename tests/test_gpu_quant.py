@@ -90,12 +90,12 @@ def test_strides_of_every_kind_are_read_in_place_or_copied(gpu, dtype):
         assert codes.shape == v.shape and torch.equal(codes, want_codes) and torch.equal(scale, want_scale)
 
 
-def test_nothing_behind_a_row_or_the_last_row_is_written(gpu):
+@pytest.mark.parametrize('m,k,n,pitch', [(37, 45, 21, 61), (9001, 45, 21, 61), (9001, 450, 300, 461)])
+def test_nothing_behind_a_row_or_the_last_row_is_written(gpu, m, k, n, pitch):
     import ctypes
     from yolo_tf_amd import _abi
     lib = _abi.load()
     rng = np.random.default_rng(6)
-    m, k, pitch = 37, 45, 61
     x = _randn(rng, m, k).to(gpu)
     codes = torch.full((m + 2, pitch), 55, dtype=torch.int8, device=gpu)
     scale = torch.full((m + 2,), -7.0, device=gpu)
@@ -106,7 +106,6 @@ def test_nothing_behind_a_row_or_the_last_row_is_written(gpu):
         out = torch.full((m + 2, pitch), 9.0, dtype=dtype, device=gpu)
         _abi.check(lib.yh_dequantize_rows(codes.data_ptr(), pitch, scale.data_ptr(), m, k, out.data_ptr(), kind, pitch, st))
         assert (out[:m, k:] == 9).all() and (out[m:] == 9).all() and (out[:m, :k] != 9).any()
-        n = 21
         w, ws = quant.quantize_rows(_randn(rng, n, k).to(gpu))
         y = torch.full((m + 2, pitch), 9.0, dtype=dtype, device=gpu)
         _abi.check(lib.yh_matmul_int8(codes.data_ptr(), 3, pitch, scale.data_ptr(), m, k, w.data_ptr(), w.stride(0), ws.data_ptr(), n,
@@ -120,7 +119,9 @@ def test_nothing_behind_a_row_or_the_last_row_is_written(gpu):
 
 # ------------------------------------------------------------------ products
 PRODUCTS = [(1, 1, 1), (1, 1024, 255), (2, 77, 3), (5, 16, 64), (16, 65, 17), (40, 64, 32), (129, 255, 130), (300, 129, 257),
-            (169, 1024, 512), (2000, 48, 27), (6000, 256, 640), (8, 6000, 20)]
+            (169, 1024, 512), (2000, 48, 27), (6000, 256, 640), (8, 6000, 20),
+            # weights kept in LDS: one to sixteen lanes a row, whole and ragged rows; large tiles with a ragged end
+            (9000, 20, 16), (5000, 100, 130), (4500, 129, 200), (4500, 256, 70), (8200, 300, 64), (12000, 300, 520), (17000, 512, 256)]
 
 
 def _layer(rng, k, n, dev):
@@ -470,6 +471,89 @@ def test_offsets_beyond_32_bits(gpu):
     for p, r in zip(quant.norm_act_backward(wide, ka), quant.norm_act_backward(x, kb)):
         assert torch.equal(p, r)
     assert torch.equal(quant.input_grad(wide, *_layer(np.random.default_rng(1), 9, k, gpu)), quant.input_grad(x, *_layer(np.random.default_rng(1), 9, k, gpu)))
+
+
+def test_pitches_beyond_the_short_offsets(gpu):
+    """Rows 2^22 elements apart and more take the loads with 64-bit offsets."""
+    rng = np.random.default_rng(34)
+    m, k, n, ld = 70, 40, 24, (1 << 22) + 16
+    x, dy = _randn(rng, m, k).to(gpu), _randn(rng, m, n).to(gpu)
+    q, s = quant.quantize_rows(x)
+    far_q = torch.empty((m, ld), dtype=torch.int8, device=gpu)[:, :k]
+    far_q.copy_(q)
+    far_dy = torch.empty((m, ld), dtype=torch.float32, device=gpu)[:, :n]
+    far_dy.copy_(dy)
+    w, ws = _layer(rng, k, n, gpu)
+    far_w = torch.empty((n, ld), dtype=torch.int8, device=gpu)[:, :k]
+    far_w.copy_(w)
+    assert torch.equal(quant.weight_grad(far_dy, far_q, s), quant.weight_grad(dy, q, s))
+    assert torch.equal(quant.input_grad(far_dy, far_w, ws), quant.input_grad(dy, w, ws))
+    # the tile form of the product: more channels than the other forms take
+    big = torch.randint(-127, 128, (m, 5000), dtype=torch.int8, device=gpu)
+    far_big = torch.empty((m, ld), dtype=torch.int8, device=gpu)[:, :5000]
+    far_big.copy_(big)
+    wb, wbs = _layer(rng, 5000, n, gpu)
+    assert torch.equal(quant.matmul_int8(far_big, wb, wbs, x_scale=s), quant.matmul_int8(big, wb, wbs, x_scale=s))
+
+
+@pytest.mark.parametrize('m,c', [(50, 40), (3000, 130), (9, 6150)])
+def test_norm_in_place(gpu, m, c):
+    """The activation may overwrite the shortcut, and dz its gradient da."""
+    import ctypes
+    from yolo_tf_amd import _abi
+    lib = _abi.load()
+    rng = np.random.default_rng(35)
+    z, res, da = (_randn(rng, m, c).to(gpu) for _ in range(3))
+    gamma, beta = (1 + 0.1 * _randn(rng, c)).to(gpu), (0.1 * _randn(rng, c)).to(gpu)
+    a, kept = quant.norm_act(z, gamma, beta, 1e-3, 0.1, residual=res)
+    dz, dgamma, dbeta = quant.norm_act_backward(da, kept)
+    st = ctypes.c_void_p(torch.cuda.current_stream(gpu).cuda_stream)
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device=gpu)
+    out, stats = res.clone(), torch.empty(2, c, device=gpu)
+    _abi.check(lib.yh_norm_act_forward(z.data_ptr(), c, out.data_ptr(), c, 0, m, c, gamma.data_ptr(), beta.data_ptr(), 1e-3, 0.1,
+                                       out.data_ptr(), c, None, 0, None, stats[0].data_ptr(), stats[1].data_ptr(), None, None, 0.0,
+                                       ws.data_ptr(), ws.numel(), st))
+    assert torch.equal(out, a)
+    grad, sums = da.clone(), torch.empty(2, c, device=gpu)
+    codes, scale = kept.kept, kept.scale
+    _abi.check(lib.yh_norm_act_backward(grad.data_ptr(), c, 0, m, c, codes.data_ptr(), kept.pitch, scale.data_ptr(), gamma.data_ptr(),
+                                        kept.invstd.data_ptr(), 0.1, grad.data_ptr(), c, sums[0].data_ptr(), sums[1].data_ptr(),
+                                        ws.data_ptr(), ws.numel(), st))
+    assert torch.equal(grad, dz) and torch.equal(sums[0], dgamma) and torch.equal(sums[1], dbeta)
+
+
+def test_rows_of_one_number_repeated(gpu):
+    """Inputs expanded along the rows or the channels (pitch 0, adjacent equal values) are read like any other."""
+    rng = np.random.default_rng(36)
+    w, ws = _layer(rng, 64, 30, gpu)
+    row, one = _randn(rng, 1, 64).to(gpu), _randn(rng, 200, 1).to(gpu)
+    for v in (row.expand(200, 64), one.expand(200, 64)):
+        assert torch.equal(quant.matmul_int8(v, w, ws), quant.matmul_int8(v.contiguous(), w, ws))
+        codes, scale = quant.quantize_rows(v.contiguous())
+        dy = _randn(rng, 1, 30).to(gpu).expand(200, 30)
+        assert torch.equal(quant.weight_grad(dy, codes, scale), quant.weight_grad(dy.contiguous(), codes, scale))
+        assert torch.equal(quant.input_grad(dy, w, ws), quant.input_grad(dy.contiguous(), w, ws))
+
+
+def test_two_threads_at_once(gpu):
+    import threading
+    rng = np.random.default_rng(37)
+    cases = [(torch.randn(5000, 256, device=gpu), *_layer(rng, 256, 96, gpu)), (torch.randn(300, 512, device=gpu), *_layer(rng, 512, 70, gpu))]
+    want = [quant.matmul_int8(*c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream(gpu)):
+            for _ in range(50):
+                if not torch.equal(quant.matmul_int8(*cases[i % 2]), want[i % 2]):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == []
 
 
 def test_empty_batches(gpu):

@@ -30,6 +30,14 @@ def test_no_cpu_path():
         quant.quantize_rows(np.zeros((3, 8), np.float32))
 
 
+def test_the_stack_options_have_no_cpu_path():
+    from yolo_tf_amd import backbone as bb
+    for option in (dict(pointwise='int8'), dict(checkpoints='int8')):
+        net = bb.Darknet19Head(2, 1, **option)
+        with pytest.raises(RuntimeError, match='no CPU path'):
+            net(torch.zeros(1, 32, 32, 3))
+
+
 def test_calls_without_a_device_say_so():
     if torch.cuda.is_available():
         pytest.skip('a HIP device is present')

@@ -472,7 +472,7 @@ int require_device()
 
 extern "C" {
 
-int yh_version(void) { return 200; }
+int yh_version(void) { return 210; }
 
 int yh_set_tuning(const yh_tuning *t)
 {
