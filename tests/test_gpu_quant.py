@@ -9,7 +9,7 @@ from tests import quant_cases as qc
 pytestmark = pytest.mark.gpu
 
 # rows and channels: one, odd, wavefront and tile edges, several row plans, a row longer than a wavefront's registers
-SHAPES = [(1, 1), (1, 1024), (3, 5), (7, 64), (65, 33), (127, 255), (33, 771), (130, 1536), (9, 6150), (4099, 32)]
+SHAPES = [(1, 1), (1, 1024), (3, 5), (7, 64), (65, 33), (127, 255), (33, 771), (130, 1536), (9, 6150), (4099, 32), (41, 2048), (21, 3001), (5, 4097)]
 
 
 def _randn(rng, *shape):
@@ -251,7 +251,7 @@ def test_non_finite_gradients_reach_what_they_touch(gpu):
 
 
 # ------------------------------------------------------------------ normalisation
-NORMS = [(1, 1), (1, 40), (2, 3), (8, 1), (7, 64), (169, 1024), (333, 255), (50, 771), (64, 1536), (5, 6150), (4100, 32), (20000, 7)]
+NORMS = [(1, 1), (1, 40), (2, 3), (8, 1), (7, 64), (169, 1024), (333, 255), (50, 771), (64, 1536), (5, 6150), (4100, 32), (20000, 7), (700, 2049), (333, 4096), (31, 4100), (3001, 1300), (9, 3001)]
 
 
 @pytest.mark.parametrize('dtype', qc.TYPES)

@@ -16,20 +16,24 @@ int pow2_at_least(int v)
 }
 
 // How a wavefront holds rows in registers: `lanes` neighbouring lanes a row, each with `vecs` vectors of V elements,
-// `lanes` vectors apart.  Four vectors a lane keep 4 KiB of loads in flight a wavefront; rows shorter than that share
-// the wavefront, with at least eight lanes (128 contiguous bytes) each.
+// `lanes` vectors apart.  `most` vectors a lane (four: 4 KiB of loads in flight a wavefront); rows shorter than that share
+// the wavefront, with at least eight lanes (128 contiguous bytes) each.  Below 2^20 lanes in all (64 wavefronts a compute
+// unit) more lanes a row fill the card better: normalisation of 10816 x 512 in float32 29.3 us with four vectors a lane, 26.8
+// with two; of 173056 x 128, with lanes enough, 57.8 and 60.2.
 struct RowPlan { int lanes, vecs; };
-RowPlan plan_row(int64_t rows, int cols, int V)
+RowPlan plan_row(int64_t rows, int cols, int V, int most)
 {
-    const int nv = (cols + V - 1) / V;
+    const int nv = (cols + V - 1) / V, all = std::min(64, pow2_at_least(nv));
     RowPlan p;
-    p.lanes = std::min(64, std::max(std::min(8, pow2_at_least(nv)), pow2_at_least((nv + 3) / 4)));
-    // few rows leave most of the card idle: as many lanes a row as there are vectors
-    if (rows * p.lanes < 64 * 1024) p.lanes = std::min(64, pow2_at_least(nv));
+    p.lanes = std::min(64, std::max(std::min(8, pow2_at_least(nv)), pow2_at_least((nv + most - 1) / most)));
+    while (p.lanes < all && rows * p.lanes < 1 << 20) p.lanes *= 2;
     p.vecs = (nv + p.lanes - 1) / p.lanes;
     return p;
 }
 
+// Row codes, written: one read of x, one write of the codes; the row waits in registers for its maximum (lanes of a row
+// exchange it by data-parallel moves).  Bound by memory: 173056 x 128 in float32 20 us (112 MB, 5.6 TB/s), 43264 x 1536 in
+// bfloat16 36.5 us (5.5 TB/s).
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_quantize(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *codes, int64_t ldc,
                                                        float *scale, int lanes)
@@ -77,7 +81,8 @@ __device__ __forceinline__ uint32_t workgroup_max(uint32_t m, uint32_t *top)
     return m;
 }
 
-// Rows longer than the registers of a wavefront: a workgroup a row, read twice (the second time from the caches).
+// Rows longer than the registers of a wavefront (eight vectors a lane: 20000 x 2048 in float32 35 us so, 41 us here): a
+// workgroup a row, read twice (the second time from the caches).
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_quantize_long(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *codes, int64_t ldc, float *scale)
 {
@@ -109,6 +114,7 @@ __global__ __launch_bounds__(kThreads) void k_quantize_long(const T *x, int64_t 
     }
 }
 
+// Row codes, read: 173056 x 128 to float32 18.8 us (111 MB, 5.9 TB/s).
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_dequantize(const int8_t *codes, int64_t ldc, const float *scale, int64_t rows, int cols,
                                                          T *out, int64_t ldo, int lanes)
@@ -158,9 +164,9 @@ ReducePlan plan_reduce(int64_t rows, int cols, int V)
 {
     const int cv = (cols + V - 1) / V;
     ReducePlan p;
-    // Up to 1024 rows one workgroup takes all rows of a slab of four vectors (64 bytes a row) and finishes by itself:
-    // the launch that adds the partials costs more than what the spread over workgroups wins (13 x 13 x 1024 bf16, both
-    // passes of a step: 22 us of kernels with it).
+    // Up to 1024 rows one workgroup takes all rows of a slab of four vectors (64 bytes a row) and finishes by itself: the
+    // launch that adds the partials costs more than what the spread over workgroups wins (forward and backward pass,
+    // 169 x 1024 in bfloat16: 18.9 us so, 24.2 with it; 1024 x 1024: 23.9 and 26.1; 4096 x 1024: 76.8 and 44.0).
     const bool alone = rows <= 1024;
     p.tx = std::min(alone ? 4 : 64, pow2_at_least(cv));
     p.ty = kThreads / p.tx;
@@ -242,6 +248,7 @@ struct NormGrads {
     }
 };
 
+// Statistics: one read of z.  346112 x 128 in float32 (177 MB): 45 us (3.9 TB/s), the adding of the partials 5 us.
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int TX, double *part,
                                                          NormStats<T> out)
@@ -321,6 +328,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats_finish(const double *pa
     if (at == 0 && (int)blockIdx.x * per + (int)threadIdx.x / lanes < cols) out.finish(c, s1, s2);
 }
 
+// The elementwise pass: z (and the shortcut) in, the activation and the checkpoint out, a row's maximum between its lanes.
+// Bound by memory: 346112 x 128 in float32 with a shortcut 97 us (577 MB, 5.9 TB/s).
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_norm_apply(const T *z, int64_t ldz, const T *res, int64_t ldr, int64_t rows, int cols,
                                                          const float *mean, const float *invstd, const float *gamma, const float *beta, float slope,
@@ -384,7 +393,83 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(const T *z, int64_t ldz
     }
 }
 
-// Rows longer than a wavefront's registers: a workgroup a row, read twice.
+// Rows over the whole workgroup, R at a time; the wavefronts exchange their maxima through LDS, in two sets of words in
+// turn, so that one barrier a turn is enough.
+template <class T, int IT, int R>
+__global__ __launch_bounds__(kThreads) void k_norm_apply_wide(const T *z, int64_t ldz, const T *res, int64_t ldr, int64_t rows, int cols,
+                                                              const float *mean, const float *invstd, const float *gamma, const float *beta, float slope,
+                                                              T *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale)
+{
+    constexpr int V = RowVec<T>::V;
+    __shared__ uint32_t top[2][R][kThreads / 64];
+    float mu[IT][V], is[IT][V], ga[IT][V], be[IT][V];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int c = (i * kThreads + threadIdx.x) * V;
+        load_vec<float, V>(mu[i], mean + c, cols - c);
+        load_vec<float, V>(is[i], invstd + c, cols - c);
+        load_vec<float, V>(ga[i], gamma + c, cols - c);
+        load_vec<float, V>(be[i], beta + c, cols - c);
+    }
+    int at = 0;
+    for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < rows; row0 += (int64_t)gridDim.x * R, at ^= 1) {
+        float v[R][IT][V], rs[R][IT][V];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const int c = (i * kThreads + threadIdx.x) * V, left = row0 + r < rows ? cols - c : 0;
+                load_vec<T, V>(v[r][i], z + (row0 + r) * ldz + c, left);
+                if (res) load_vec<T, V>(rs[r][i], res + (row0 + r) * ldr + c, left);
+            }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    v[r][i][j] = (v[r][i][j] - mu[i][j]) * is[i][j];
+                    if ((i * kThreads + (int)threadIdx.x) * V + j < cols) m = max(m, __float_as_uint(v[r][i][j]) & 0x7fffffffu);
+                }
+            m = row_max(m, 64);
+            if ((threadIdx.x & 63) == 0) top[at][r][threadIdx.x >> 6] = m;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + r;
+            if (row >= rows) break;
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < kThreads / 64; ++i) m = max(m, top[at][r][i]);
+            const RowScale k = row_scale(m, (float)kKeptMax);
+            if (kept && threadIdx.x == 0) scale[row] = k.s;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const int c = (i * kThreads + threadIdx.x) * V;
+                uint32_t w[V / 4], b[V];
+                float o[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float u = v[r][i][j] * ga[i][j] + be[i][j];
+                    const bool up = u > 0.0f;
+                    o[j] = up ? u : slope * u;
+                    if (res) o[j] += rs[r][i][j];
+                    b[j] = ((k.live ? code_bits(v[r][i][j], k.r) : 0u) << 1) | (up ? 1u : 0u);
+                }
+                store_vec<T, V>(a + row * lda + c, o, cols - c);
+                if (kept) {
+#pragma unroll
+                    for (int j = 0; j < V; j += 4) w[j / 4] = pack4(b[j], b[j + 1], b[j + 2], b[j + 3]);
+                    store_bytes<V>(kept + row * ldk + c, w, cols - c);
+                }
+            }
+        }
+    }
+}
+
+// Rows of any length: a workgroup a row, read twice.
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_apply_long(const T *z, int64_t ldz, const T *res, int64_t ldr, int64_t rows, int cols,
                                                               const float *mean, const float *invstd, const float *gamma, const float *beta, float slope,
@@ -437,6 +522,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply_long(const T *z, int64_
 __device__ __forceinline__ float kept_code(uint32_t w, int i) { return (float)((int8_t)(w >> (8 * i)) >> 1); }
 __device__ __forceinline__ bool kept_side(uint32_t w, int i) { return (w >> (8 * i)) & 1u; }
 
+// Sums of the backward pass: da and the checkpoint in.  346112 x 128 in float32 (223 MB): 55 us (4.0 TB/s).
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
                                                              int64_t rows, int cols, float slope, int TX, double *part,
@@ -498,6 +584,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_finish(const double *par
     if (at == 0 && (int)blockIdx.x * per + (int)threadIdx.x / lanes < cols) out.finish(c, b, g);
 }
 
+// Input gradient: da and the checkpoint again, dz out.  346112 x 128 in float32 (400 MB): 68 us (5.9 TB/s).
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
                                                               int64_t rows, int cols, float slope, const float *gamma, const float *invstd,
@@ -558,13 +645,13 @@ void with_type(int32_t type, F f)
     else f((_Float16)0.0f);
 }
 
-// Calls f.template operator()<IT>() is not available before C++20: the vector counts are spelled out.
+// The kernels' vector counts.
 #define YH_WITH_VECS(vecs, CALL)            \
     do {                                    \
         if ((vecs) <= 1) { CALL(1); }       \
         else if ((vecs) <= 2) { CALL(2); }  \
         else if ((vecs) <= 4) { CALL(4); }  \
-        else { CALL(6); }                   \
+        else { CALL(8); }                   \
     } while (0)
 
 unsigned row_blocks(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 1 << 20); }
@@ -577,8 +664,8 @@ hipError_t launch_quantize(const Rows &x, int64_t rows, int32_t cols, int8_t *co
     with_type(x.type, [&](auto t) {
         using T = decltype(t);
         const T *p = static_cast<const T *>(x.p);
-        const RowPlan r = plan_row(rows, cols, RowVec<T>::V);
-        if (r.vecs > 6) {
+        const RowPlan r = plan_row(rows, cols, RowVec<T>::V, 4);
+        if (r.vecs > 8) {
             k_quantize_long<T><<<dim3(row_blocks(rows)), kThreads, 0, st>>>(p, rows, cols, x.ld, codes, ldc, scale);
             return;
         }
@@ -595,7 +682,7 @@ hipError_t launch_dequantize(const int8_t *codes, int64_t ldc, const float *scal
 {
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        const RowPlan r = plan_row(rows, cols, RowVec<T>::V);
+        const RowPlan r = plan_row(rows, cols, RowVec<T>::V, 4);
         const unsigned blocks = waves_to_blocks((rows * r.lanes + 63) / 64);
 #define CALL(IT) k_dequantize<T, IT><<<dim3(blocks), kThreads, 0, st>>>(codes, ldc, scale, rows, cols, static_cast<T *>(out), ldo, r.lanes)
         YH_WITH_VECS(r.vecs, CALL);
@@ -624,16 +711,34 @@ hipError_t launch_norm_forward(const Rows &z, const Rows &res, int64_t rows, int
         const int lanes = d.blocks > 64 ? kThreads : 64;
         if (d.blocks > 1)
             k_norm_stats_finish<T><<<dim3((cols * lanes + kThreads - 1) / kThreads), kThreads, 0, st>>>(part, d.blocks, cols, lanes, out);
-        const RowPlan r = plan_row(rows, cols, RowVec<T>::V);
-        if (r.vecs > 6) {
+        // Per channel four numbers stay in registers, so a lane holds at most 16 channels and beyond a wavefront's 1024 the
+        // workgroup takes the row (20000 x 2048 in float32: 138 us in all, 171 by the kernel for any length; 20000 x 1536 in
+        // bfloat16 77 us, 101 with 24 channels a lane).  With 16-bit vectors one a lane is best where lanes are enough
+        // (173056 x 256 with a shortcut: 94 us, two: 104, four: 121), with float32 four.
+        constexpr int V = RowVec<T>::V, kMost = 16 / V, kLane = V == 4 ? 4 : 1, R = 2;
+        const RowPlan r = plan_row(rows, cols, V, kLane);
+        if (cols > kThreads * 16) {
             k_norm_apply_long<T><<<dim3(row_blocks(rows)), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope,
                                                                             static_cast<T *>(a), lda, kept, ldk, scale);
+            return;
+        }
+        if (r.vecs > kMost) {
+            const int per = (cols + kThreads * V - 1) / (kThreads * V);
+            const unsigned blocks = (unsigned)std::min<int64_t>(2048, (rows + R - 1) / R);
+#define CALL(IT) k_norm_apply_wide<T, IT, R><<<dim3(blocks), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope, \
+                                                                               static_cast<T *>(a), lda, kept, ldk, scale)
+            if (per <= 1) CALL(1);
+            else if (per <= 2) CALL(2);
+            else if constexpr (kMost == 4) CALL(4);
+#undef CALL
             return;
         }
         const unsigned blocks = std::min(2048u, waves_to_blocks((rows * r.lanes + 63) / 64));
 #define CALL(IT) k_norm_apply<T, IT><<<dim3(blocks), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope, \
                                                                         static_cast<T *>(a), lda, kept, ldk, scale, r.lanes, (int64_t)blocks * (kThreads / 64))
-        YH_WITH_VECS(r.vecs, CALL);
+        if (r.vecs <= 1) CALL(1);
+        else if (r.vecs <= 2) CALL(2);
+        else if constexpr (kMost == 4) CALL(4);
 #undef CALL
     });
     return hipGetLastError();
@@ -653,14 +758,16 @@ hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, cons
         const int lanes = d.blocks > 64 ? kThreads : 64;
         if (d.blocks > 1)
             k_norm_grad_finish<<<dim3((cols * lanes + kThreads - 1) / kThreads), kThreads, 0, st>>>(part, d.blocks, cols, lanes, out);
-        const RowPlan r = plan_row(rows, cols, RowVec<T>::V);
-        const int vecs = std::min(4, r.vecs), step = (vecs <= 1 ? 1 : vecs <= 2 ? 2 : 4) * r.lanes * RowVec<T>::V;
+        // the forward pass's lanes; 16 channels at most, further ones in workgroups of their own
+        constexpr int V = RowVec<T>::V, kMost = 16 / V, kLane = V == 4 ? 4 : 1;
+        const RowPlan r = plan_row(rows, cols, V, kLane);
+        const int vecs = std::min(kMost, r.vecs), step = (vecs <= 1 ? 1 : vecs <= 2 ? 2 : 4) * r.lanes * V;
         const unsigned blocks = std::min(2048u, waves_to_blocks((rows * r.lanes + 63) / 64));
 #define CALL(IT) k_norm_grad_apply<T, IT><<<dim3(blocks, (cols + step - 1) / step), kThreads, 0, st>>>( \
             p, da.ld, kept, ldk, scale, rows, cols, slope, gamma, invstd, dgamma, dbeta, static_cast<T *>(dz), lddz, r.lanes, (int64_t)blocks * (kThreads / 64))
         if (vecs <= 1) CALL(1);
         else if (vecs <= 2) CALL(2);
-        else CALL(4);
+        else if constexpr (kMost == 4) CALL(4);
 #undef CALL
     });
     return hipGetLastError();
