@@ -53,17 +53,10 @@ __device__ __forceinline__ v4i load_at16(Buffer b, uint32_t lane, uint32_t unifo
 
 __device__ __forceinline__ v4i load_chunk(const int8_t *p, int left)
 {
-    v4i v = {0, 0, 0, 0};
-    if (left >= 16) {
-        const LooseBytes<16>::type t = *reinterpret_cast<const LooseBytes<16>::type *>(p);
-        __builtin_memcpy(&v, &t, 16);
-    } else if (left > 0) {
-        uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 15; ++i)
-            if (i < left) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
-        __builtin_memcpy(&v, w, 16);
-    }
+    uint32_t w[4];
+    load_bytes<16>(w, p, left);
+    v4i v;
+    __builtin_memcpy(&v, w, 16);
     return v;
 }
 
@@ -228,10 +221,9 @@ __device__ __forceinline__ v4i load_elements(const TX *p, int left)
         const LooseBytes<16>::type t = *reinterpret_cast<const LooseBytes<16>::type *>(p);
         __builtin_memcpy(&v, &t, 16);
     } else if (!kWhole && left > 0) {
-        TX t[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) t[i] = i < left ? p[i] : (TX)0;
-        __builtin_memcpy(&v, t, 16);
+        uint32_t w[4];
+        load_end<sizeof(TX), 4>(w, p, left * (int)sizeof(TX));
+        __builtin_memcpy(&v, w, 16);
     }
     return v;
 }
@@ -643,10 +635,7 @@ struct AlongOperand {
         for (int n = 0; n < N; ++n) {
             const int u = threadIdx.x + n * kThreads, c = u % C * E;
             const T *p = base + min((int64_t)(u / C), na - 1 - a0) * ld + r + c;
-            T w[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) w[e] = c + e < left ? p[e] : (T)0.0f;
-            __builtin_memcpy(&v[n], w, 16);
+            v[n] = load_elements<T, false>(p, left - c);
         }
     }
     __device__ __forceinline__ void store(int8_t *lds) const

@@ -56,19 +56,75 @@ template <class T> struct RowVec { static constexpr int V = 16 / (int)sizeof(T);
 template <class T, int V> struct Loose { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)), may_alias)); };
 template <int B> struct LooseBytes { typedef uint32_t type __attribute__((ext_vector_type(B / 4), aligned(1), may_alias)); };
 template <> struct LooseBytes<4> { typedef uint32_t type __attribute__((aligned(1), may_alias)); };
+template <> struct LooseBytes<2> { typedef uint16_t type __attribute__((aligned(1), may_alias)); };
+
+template <int B>
+__device__ __forceinline__ typename LooseBytes<B>::type loose_load(const uint8_t *p) { return *reinterpret_cast<const typename LooseBytes<B>::type *>(p); }
+template <int B>
+__device__ __forceinline__ void loose_store(uint8_t *p, typename LooseBytes<B>::type v) { *reinterpret_cast<typename LooseBytes<B>::type *>(p) = v; }
+
+// A row's end: `bytes` of it (0 < bytes < 4 W, whole elements of E bytes) as words, zeros behind.  One access a bit of
+// `bytes`, all under way together (element by element, each under a condition of its own, a lane's end took as long as
+// all the rest of a short call).
+template <int E, int W>
+__device__ __forceinline__ void load_end(uint32_t (&w)[W], const void *from, int bytes)
+{
+    const uint8_t *p = static_cast<const uint8_t *>(from);
+    uint32_t a[2] = {0, 0}, b = 0, c = 0, d = 0;
+    if (W > 2 && (bytes & 8)) {
+        const LooseBytes<8>::type t = loose_load<8>(p);
+        a[0] = t[0], a[1] = t[1];
+    }
+    if (W > 1 && (bytes & 4)) b = loose_load<4>(p + (bytes & 8));
+    if (E <= 2 && (bytes & 2)) c = loose_load<2>(p + (bytes & 12));
+    if (E <= 1 && (bytes & 1)) d = p[bytes & 14];
+    c |= d << ((bytes & 2) * 8);
+    const uint32_t lo = bytes & 4 ? b : c, hi = bytes & 4 ? c : 0;
+    const bool far = bytes & 8;
+    w[0] = far ? a[0] : lo;
+    if constexpr (W > 1) w[1] = far ? a[1] : hi;
+    if constexpr (W > 2) w[2] = far ? lo : 0, w[3] = far ? hi : 0;
+}
+template <int E, int W>
+__device__ __forceinline__ void store_end(void *to, const uint32_t (&w)[W], int bytes)
+{
+    uint8_t *p = static_cast<uint8_t *>(to);
+    uint32_t lo = w[0], hi = W > 1 ? w[W > 1 ? 1 : 0] : 0;
+    if constexpr (W > 2) {
+        if (bytes & 8) {
+            loose_store<8>(p, LooseBytes<8>::type{w[0], w[1]});
+            lo = w[2], hi = w[3];
+        }
+    }
+    if (W > 1 && (bytes & 4)) loose_store<4>(p + (bytes & 8), lo);
+    const uint32_t c = bytes & 4 ? hi : lo;
+    if (E <= 2 && (bytes & 2)) loose_store<2>(p + (bytes & 12), (uint16_t)c);
+    if (E <= 1 && (bytes & 1)) p[bytes & 14] = (uint8_t)(c >> ((bytes & 2) * 8));
+}
 
 // `left` elements of a row from p on, as float32; what lies behind the row's end is not read and comes back zero.
 // The address is aligned to an element only: rows of odd length start anywhere.
 template <class T, int V>
 __device__ __forceinline__ void load_vec(float (&out)[V], const T *p, int left)
 {
-    if (left >= V) {
+    constexpr int W = V * (int)sizeof(T) / 4;
+    if constexpr (W > 4) {
+        float lo[V / 2], hi[V / 2];
+        load_vec<T, V / 2>(lo, p, left);
+        load_vec<T, V / 2>(hi, p + V / 2, left - V / 2);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) out[i] = lo[i], out[V / 2 + i] = hi[i];
+    } else if (left >= V) {
         const typename Loose<T, V>::type t = *reinterpret_cast<const typename Loose<T, V>::type *>(p);
 #pragma unroll
         for (int i = 0; i < V; ++i) out[i] = (float)t[i];
     } else {
+        uint32_t w[W] = {};
+        if (left > 0) load_end<sizeof(T), W>(w, p, left * (int)sizeof(T));
+        T t[V];
+        __builtin_memcpy(t, w, 4 * W);
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = i < left ? (float)p[i] : 0.0f;
+        for (int i = 0; i < V; ++i) out[i] = (float)t[i];
     }
 }
 
@@ -76,15 +132,16 @@ __device__ __forceinline__ void load_vec(float (&out)[V], const T *p, int left)
 template <class T, int V>
 __device__ __forceinline__ void store_vec(T *p, const float (&v)[V], int left)
 {
+    constexpr int W = V * (int)sizeof(T) / 4;
+    typename Loose<T, V>::type t;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = (T)v[i];
     if (left >= V) {
-        typename Loose<T, V>::type t;
-#pragma unroll
-        for (int i = 0; i < V; ++i) t[i] = (T)v[i];
         *reinterpret_cast<typename Loose<T, V>::type *>(p) = t;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < left) p[i] = (T)v[i];
+    } else if (left > 0) {
+        uint32_t w[W];
+        __builtin_memcpy(w, &t, 4 * W);
+        store_end<sizeof(T), W>(p, w, left * (int)sizeof(T));
     }
 }
 
@@ -95,10 +152,8 @@ __device__ __forceinline__ void store_bytes(int8_t *p, const uint32_t (&w)[V / 4
         typename LooseBytes<V>::type t;
         __builtin_memcpy(&t, w, V);
         *reinterpret_cast<typename LooseBytes<V>::type *>(p) = t;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < left) p[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+    } else if (left > 0) {
+        store_end<1, V / 4>(p, w, left);
     }
 }
 
@@ -111,9 +166,7 @@ __device__ __forceinline__ void load_bytes(uint32_t (&w)[V / 4], const int8_t *p
     } else {
 #pragma unroll
         for (int i = 0; i < V / 4; ++i) w[i] = 0;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < left) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
+        if (left > 0) load_end<1, V / 4>(w, p, left);
     }
 }
 
