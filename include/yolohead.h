@@ -383,7 +383,8 @@ int yh_loss_with_grad(const yh_head_config *cfg, const float *const *heads, cons
  *    to the next: at least the number of channels for outputs, not negative for
  *    inputs (0: one row for all).  A pointer is aligned to its element, nothing
  *    more is asked; multiples of 16 bytes are faster.  What lies between the rows
- *    or behind the last one is neither read nor written.
+ *    is never written and has no effect on a result, but it is read as memory; behind
+ *    the last row nothing is touched.
  *  - x, y, dy, dx, z, a, da, dz are YH_FLOAT32, YH_BFLOAT16 or YH_FLOAT16 (one type
  *    a call unless said otherwise); scales, vectors per channel, dw and db are
  *    float32.  Results of 16 bits are rounded once from float32.

@@ -170,6 +170,15 @@ __device__ __forceinline__ void load_bytes(uint32_t (&w)[V / 4], const int8_t *p
     }
 }
 
+// Rows of a matrix, from the first on, in which a vector of V elements that begins inside of the row may be read whole: it
+// runs over into the pitch or the next rows, and the matrix goes on for as long.
+inline int64_t spare_rows(int64_t rows, int64_t ld, int V) { return ld > 0 ? rows - (V - 2 + ld) / ld : 0; }
+// Elements that may be read from column c on, of a row of `cols`; those beyond `cols` are somebody else's.
+__device__ __forceinline__ int left_of(int64_t row, int64_t rows, int64_t spare, int cols, int c, int V)
+{
+    return row >= rows ? 0 : (row < spare ? (cols + V - 1) & -V : cols) - c;
+}
+
 __device__ __forceinline__ float code_value(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 
 // Round-half-even of the exact product x * r, |x * r| <= 127.0001: the fused multiply-add rounds once, to the unit of

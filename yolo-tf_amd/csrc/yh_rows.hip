@@ -36,19 +36,26 @@ RowPlan plan_row(int64_t rows, int cols, int V, int most)
 // bfloat16 36.5 us (5.5 TB/s).
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_quantize(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *codes, int64_t ldc,
-                                                       float *scale, int lanes)
+                                                       float *scale, int lanes, int64_t spare)
 {
     constexpr int V = RowVec<T>::V;
     const int lane = threadIdx.x & 63, sub = lane & (lanes - 1);
     const int64_t wave = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
     const int64_t row = wave * (64 / lanes) + lane / lanes;
+    const int read = left_of(row, rows, spare, cols, 0, V);
     float v[IT][V];
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const int c = (i * lanes + sub) * V;
-        load_vec<T, V>(v[i], x + row * ldx + c, row < rows ? cols - c : 0);
+        load_vec<T, V>(v[i], x + row * ldx + c, read - c);
     }
+    if (cols % V)
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if ((i * lanes + sub) * V + j >= cols) v[i][j] = 0.0f;
 #pragma unroll
     for (int i = 0; i < IT; ++i)
 #pragma unroll
@@ -117,7 +124,7 @@ __global__ __launch_bounds__(kThreads) void k_quantize_long(const T *x, int64_t 
 // Row codes, read: 173056 x 128 to float32 18.8 us (111 MB, 5.9 TB/s).
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_dequantize(const int8_t *codes, int64_t ldc, const float *scale, int64_t rows, int cols,
-                                                         T *out, int64_t ldo, int lanes)
+                                                         T *out, int64_t ldo, int lanes, int64_t spare)
 {
     constexpr int V = RowVec<T>::V;
     const int lane = threadIdx.x & 63, sub = lane & (lanes - 1);
@@ -125,12 +132,13 @@ __global__ __launch_bounds__(kThreads) void k_dequantize(const int8_t *codes, in
     const int64_t row = wave * (64 / lanes) + lane / lanes;
     if (row >= rows) return;
     const float s = scale[row];
+    const int read = left_of(row, rows, spare, cols, 0, V);
     for (int base = 0; base < cols; base += IT * lanes * V) {
         uint32_t w[IT][V / 4];
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int c = base + (i * lanes + sub) * V;
-            load_bytes<V>(w[i], codes + row * ldc + c, cols - c);
+            load_bytes<V>(w[i], codes + row * ldc + c, read - c);
         }
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
@@ -250,7 +258,7 @@ struct NormGrads {
 
 // Statistics: one read of z.  346112 x 128 in float32 (177 MB): 45 us (3.9 TB/s), the adding of the partials 5 us.
 template <class T>
-__global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int TX, double *part,
+__global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int64_t spare, int TX, double *part,
                                                          NormStats<T> out)
 {
     constexpr int V = RowVec<T>::V, U = 4;
@@ -261,8 +269,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t row
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
     load_vec<T, V>(first, z + c, left);
+    const int64_t step = (int64_t)gridDim.x * U * TY, rows_whole = left >= V ? rows : spare;
     const T *p = z + c;
-    const int64_t step = (int64_t)gridDim.x * U * TY;
     const auto add = [&](const float (&v)[V]) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -272,15 +280,15 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t row
         }
     };
     int64_t r = (int64_t)blockIdx.x * U * TY + ty;
-    if (left >= V)                                   // whole vectors, whole groups of rows: nothing to ask in the loop
-        for (; r + (U - 1) * TY < rows; r += step) {
+    if (left > 0)                                    // whole vectors, whole groups of rows: nothing to ask in the loop
+        for (; r + (U - 1) * TY < rows_whole; r += step) {
             float v[U][V];
 #pragma unroll
             for (int i = 0; i < U; ++i) load_vec<T, V>(v[i], p + (r + i * TY) * ldz, V);
 #pragma unroll
             for (int i = 0; i < U; ++i) add(v[i]);
         }
-    for (; r < rows; r += step) {                    // rows past the end are read as the last one and left out
+    for (; left > 0 && r < rows; r += step) {        // rows past the end are read as the last one and left out
         float v[U][V];
 #pragma unroll
         for (int i = 0; i < U; ++i) load_vec<T, V>(v[i], p + min(r + i * TY, rows - 1) * ldz, left);
@@ -333,7 +341,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats_finish(const double *pa
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_norm_apply(const T *z, int64_t ldz, const T *res, int64_t ldr, int64_t rows, int cols,
                                                          const float *mean, const float *invstd, const float *gamma, const float *beta, float slope,
-                                                         T *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale, int lanes, int64_t waves)
+                                                         T *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale, int64_t spare, int lanes, int64_t waves)
 {
     constexpr int V = RowVec<T>::V;
     const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), rpw = 64 / lanes;
@@ -350,12 +358,13 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(const T *z, int64_t ldz
     for (int64_t g = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); g * rpw < rows; g += waves) {
         const int64_t row = g * rpw + lane / lanes;
         const bool in = row < rows;
+        const int read = left_of(row, rows, spare, cols, 0, V);
         float v[IT][V], rs[IT][V];
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int c = (i * lanes + sub) * V;
-            load_vec<T, V>(v[i], z + row * ldz + c, in ? cols - c : 0);
-            if (res) load_vec<T, V>(rs[i], res + row * ldr + c, in ? cols - c : 0);
+            load_vec<T, V>(v[i], z + row * ldz + c, read - c);
+            if (res) load_vec<T, V>(rs[i], res + row * ldr + c, read - c);
         }
         uint32_t m = 0;
 #pragma unroll
@@ -398,7 +407,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(const T *z, int64_t ldz
 template <class T, int IT, int R>
 __global__ __launch_bounds__(kThreads) void k_norm_apply_wide(const T *z, int64_t ldz, const T *res, int64_t ldr, int64_t rows, int cols,
                                                               const float *mean, const float *invstd, const float *gamma, const float *beta, float slope,
-                                                              T *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale)
+                                                              T *a, int64_t lda, int8_t *kept, int64_t ldk, float *scale, int64_t spare)
 {
     constexpr int V = RowVec<T>::V;
     __shared__ uint32_t top[2][R][kThreads / 64];
@@ -418,7 +427,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply_wide(const T *z, int64_
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
-                const int c = (i * kThreads + threadIdx.x) * V, left = row0 + r < rows ? cols - c : 0;
+                const int c = (i * kThreads + threadIdx.x) * V, left = left_of(row0 + r, rows, spare, cols, c, V);
                 load_vec<T, V>(v[r][i], z + (row0 + r) * ldz + c, left);
                 if (res) load_vec<T, V>(rs[r][i], res + (row0 + r) * ldr + c, left);
             }
@@ -525,7 +534,7 @@ __device__ __forceinline__ bool kept_side(uint32_t w, int i) { return (w >> (8 *
 // Sums of the backward pass: da and the checkpoint in.  346112 x 128 in float32 (223 MB): 55 us (4.0 TB/s).
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
-                                                             int64_t rows, int cols, float slope, int TX, double *part,
+                                                             int64_t rows, int cols, float slope, int64_t spare, int TX, double *part,
                                                              NormGrads out)
 {
     constexpr int V = RowVec<T>::V, U = 4;
@@ -534,7 +543,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_
     double s1[V], s2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
-    const int64_t step = (int64_t)gridDim.x * U * TY;
+    const int64_t step = (int64_t)gridDim.x * U * TY, rows_whole = left >= V ? rows : spare;
     const auto add = [&](const float (&v)[V], const uint32_t (&w)[V / 4], float s) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -545,8 +554,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_
         }
     };
     int64_t r = (int64_t)blockIdx.x * U * TY + ty;
-    if (left >= V)
-        for (; r + (U - 1) * TY < rows; r += step) {
+    if (left > 0)
+        for (; r + (U - 1) * TY < rows_whole; r += step) {
             float v[U][V], s[U];
             uint32_t w[U][V / 4];
 #pragma unroll
@@ -559,7 +568,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_
 #pragma unroll
             for (int i = 0; i < U; ++i) add(v[i], w[i], s[i]);
         }
-    for (; r < rows; r += step) {
+    for (; left > 0 && r < rows; r += step) {
         float v[U][V], s[U];
         uint32_t w[U][V / 4];
 #pragma unroll
@@ -588,7 +597,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_finish(const double *par
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
                                                               int64_t rows, int cols, float slope, const float *gamma, const float *invstd,
-                                                              const float *dgamma, const float *dbeta, T *dz, int64_t ldz, int lanes, int64_t waves)
+                                                              const float *dgamma, const float *dbeta, T *dz, int64_t ldz, int64_t spare, int lanes, int64_t waves)
 {
     constexpr int V = RowVec<T>::V;
     const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), rpw = 64 / lanes;
@@ -613,14 +622,15 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64
     for (int64_t w0 = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); w0 * rpw < rows; w0 += waves) {
         const int64_t row = w0 * rpw + lane / lanes;
         if (row >= rows) continue;
+        const int read = left_of(row, rows, spare, cols, 0, V);
         float v[IT][V];
         uint32_t w[IT][V / 4];
         const float s = scale[row];
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int c = c0 + (i * lanes + sub) * V;
-            load_vec<T, V>(v[i], da + row * ldd + c, cols - c);
-            load_bytes<V>(w[i], kept + row * ldk + c, cols - c);
+            load_vec<T, V>(v[i], da + row * ldd + c, read - c);
+            load_bytes<V>(w[i], kept + row * ldk + c, read - c);
         }
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
@@ -670,7 +680,7 @@ hipError_t launch_quantize(const Rows &x, int64_t rows, int32_t cols, int8_t *co
             return;
         }
         const unsigned blocks = waves_to_blocks((rows * r.lanes + 63) / 64);
-#define CALL(IT) k_quantize<T, IT><<<dim3(blocks), kThreads, 0, st>>>(p, rows, cols, x.ld, codes, ldc, scale, r.lanes)
+#define CALL(IT) k_quantize<T, IT><<<dim3(blocks), kThreads, 0, st>>>(p, rows, cols, x.ld, codes, ldc, scale, r.lanes, spare_rows(rows, x.ld, RowVec<T>::V))
         YH_WITH_VECS(r.vecs, CALL);
 #undef CALL
     });
@@ -684,7 +694,7 @@ hipError_t launch_dequantize(const int8_t *codes, int64_t ldc, const float *scal
         using T = decltype(t);
         const RowPlan r = plan_row(rows, cols, RowVec<T>::V, 4);
         const unsigned blocks = waves_to_blocks((rows * r.lanes + 63) / 64);
-#define CALL(IT) k_dequantize<T, IT><<<dim3(blocks), kThreads, 0, st>>>(codes, ldc, scale, rows, cols, static_cast<T *>(out), ldo, r.lanes)
+#define CALL(IT) k_dequantize<T, IT><<<dim3(blocks), kThreads, 0, st>>>(codes, ldc, scale, rows, cols, static_cast<T *>(out), ldo, r.lanes, spare_rows(rows, ldc, RowVec<T>::V))
         YH_WITH_VECS(r.vecs, CALL);
 #undef CALL
     });
@@ -707,7 +717,7 @@ hipError_t launch_norm_forward(const Rows &z, const Rows &res, int64_t rows, int
         const T *p = static_cast<const T *>(z.p), *q = static_cast<const T *>(res.p);
         const ReducePlan d = plan_reduce(rows, cols, RowVec<T>::V);
         const NormStats<T> out{p, rows, eps, momentum, mean, invstd, running_mean, running_var};
-        k_norm_stats<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, rows, cols, z.ld, d.tx, part, out);
+        k_norm_stats<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, rows, cols, z.ld, spare_rows(rows, z.ld, RowVec<T>::V), d.tx, part, out);
         const int lanes = d.blocks > 64 ? kThreads : 64;
         if (d.blocks > 1)
             k_norm_stats_finish<T><<<dim3((cols * lanes + kThreads - 1) / kThreads), kThreads, 0, st>>>(part, d.blocks, cols, lanes, out);
@@ -716,6 +726,7 @@ hipError_t launch_norm_forward(const Rows &z, const Rows &res, int64_t rows, int
         // bfloat16 77 us, 101 with 24 channels a lane).  With 16-bit vectors one a lane is best where lanes are enough
         // (173056 x 256 with a shortcut: 94 us, two: 104, four: 121), with float32 four.
         constexpr int V = RowVec<T>::V, kMost = 16 / V, kLane = V == 4 ? 4 : 1, R = 2;
+        const int64_t spare = std::min(spare_rows(rows, z.ld, V), q ? spare_rows(rows, res.ld, V) : rows);
         const RowPlan r = plan_row(rows, cols, V, kLane);
         if (cols > kThreads * 16) {
             k_norm_apply_long<T><<<dim3(row_blocks(rows)), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope,
@@ -726,7 +737,7 @@ hipError_t launch_norm_forward(const Rows &z, const Rows &res, int64_t rows, int
             const int per = (cols + kThreads * V - 1) / (kThreads * V);
             const unsigned blocks = (unsigned)std::min<int64_t>(2048, (rows + R - 1) / R);
 #define CALL(IT) k_norm_apply_wide<T, IT, R><<<dim3(blocks), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope, \
-                                                                               static_cast<T *>(a), lda, kept, ldk, scale)
+                                                                               static_cast<T *>(a), lda, kept, ldk, scale, spare)
             if (per <= 1) CALL(1);
             else if (per <= 2) CALL(2);
             else if constexpr (kMost == 4) CALL(4);
@@ -735,7 +746,7 @@ hipError_t launch_norm_forward(const Rows &z, const Rows &res, int64_t rows, int
         }
         const unsigned blocks = std::min(2048u, waves_to_blocks((rows * r.lanes + 63) / 64));
 #define CALL(IT) k_norm_apply<T, IT><<<dim3(blocks), kThreads, 0, st>>>(p, z.ld, q, res.ld, rows, cols, mean, invstd, gamma, beta, slope, \
-                                                                        static_cast<T *>(a), lda, kept, ldk, scale, r.lanes, (int64_t)blocks * (kThreads / 64))
+                                                                        static_cast<T *>(a), lda, kept, ldk, scale, spare, r.lanes, (int64_t)blocks * (kThreads / 64))
         if (r.vecs <= 1) CALL(1);
         else if (r.vecs <= 2) CALL(2);
         else if constexpr (kMost == 4) CALL(4);
@@ -754,7 +765,8 @@ hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, cons
         const T *p = static_cast<const T *>(da.p);
         const ReducePlan d = plan_reduce(rows, cols, RowVec<T>::V);
         const NormGrads out{dgamma, dbeta};
-        k_norm_grad_sums<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, da.ld, kept, ldk, scale, rows, cols, slope, d.tx, part, out);
+        const int64_t spare = std::min(spare_rows(rows, da.ld, RowVec<T>::V), spare_rows(rows, ldk, RowVec<T>::V));
+        k_norm_grad_sums<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, da.ld, kept, ldk, scale, rows, cols, slope, spare, d.tx, part, out);
         const int lanes = d.blocks > 64 ? kThreads : 64;
         if (d.blocks > 1)
             k_norm_grad_finish<<<dim3((cols * lanes + kThreads - 1) / kThreads), kThreads, 0, st>>>(part, d.blocks, cols, lanes, out);
@@ -764,7 +776,7 @@ hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, cons
         const int vecs = std::min(kMost, r.vecs), step = (vecs <= 1 ? 1 : vecs <= 2 ? 2 : 4) * r.lanes * V;
         const unsigned blocks = std::min(2048u, waves_to_blocks((rows * r.lanes + 63) / 64));
 #define CALL(IT) k_norm_grad_apply<T, IT><<<dim3(blocks, (cols + step - 1) / step), kThreads, 0, st>>>( \
-            p, da.ld, kept, ldk, scale, rows, cols, slope, gamma, invstd, dgamma, dbeta, static_cast<T *>(dz), lddz, r.lanes, (int64_t)blocks * (kThreads / 64))
+            p, da.ld, kept, ldk, scale, rows, cols, slope, gamma, invstd, dgamma, dbeta, static_cast<T *>(dz), lddz, spare, r.lanes, (int64_t)blocks * (kThreads / 64))
         if (vecs <= 1) CALL(1);
         else if (vecs <= 2) CALL(2);
         else if constexpr (kMost == 4) CALL(4);
