@@ -211,8 +211,8 @@ __global__ __launch_bounds__(kThreads) void k_int8_tile(const int8_t *x, int64_t
     }
 }
 
-// 16 bytes of a row's elements from p on, `left` of them inside of the row; zeros behind.
-template <class TX, bool kWhole>
+// 16 bytes of a row's elements from p on, `left` of them to be read; zeros behind.
+template <class TX, bool kWhole = false>                   // kWhole: 16 bytes or nothing
 __device__ __forceinline__ v4i load_elements(const TX *p, int left)
 {
     constexpr int V = 16 / (int)sizeof(TX);
@@ -228,12 +228,21 @@ __device__ __forceinline__ v4i load_elements(const TX *p, int left)
     return v;
 }
 
+// Zeros in the place of the elements from `left` on.
+template <class TX, int V>
+__device__ __forceinline__ void clear_end(TX (&t)[V], int left)
+{
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j >= left) t[j] = (TX)0;
+}
+
 // ---- the same from float rows: codes taken on the way --------------------------
 // Reading x once and writing y once is all the product has to move, so where it can the product takes the codes itself
 // and they stay in LDS.  A wavefront turns 16 rows into codes at a time: `lanes` (4 to 16) neighbouring lanes a row, four
 // vectors of 16 bytes each, so rows of up to 1024 bytes, and leaves them in LDS rows of k64 + 16 bytes (k64: K rounded up to 64, zeros
 // behind K; the 16 bytes shift each row by a bank group, so that 16 rows are read without a conflict).
-template <class TX, int G, bool kWhole>                  // kWhole: K is a multiple of V
+template <class TX, int G, bool kWhole>                  // kWhole: K is a multiple of 16
 struct CodeRows {
     static constexpr int V = 16 / (int)sizeof(TX);
     v4i raw[G][4];                                       // G = lanes / 4 passes of 64 / lanes rows, as they are in memory
@@ -380,23 +389,54 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_int8_rows(const TX *x, int64
     }
 }
 
-// Four rows of a workgroup's 16 a wavefront, each by all its lanes: codes at lx, scales at ls (k_int8_few).
-template <class TX, bool kWhole>
-__device__ __forceinline__ void code_four_rows(const TX *x, int64_t ldx, const float *, int64_t first, int64_t rows, int k, int k64,
-                                               int8_t *lx, float *ls, int8_t *codes, int64_t ldc, float *scale)
+// The 16 rows of codes from LDS (pitch `pitch`) to memory, by the workgroup.
+__device__ __forceinline__ void codes_out(const int8_t *lx, int pitch, int64_t first, int64_t rows, int k, int8_t *codes, int64_t ldc)
 {
-    constexpr int V = RowVec<TX>::V, IT = 4;
+    const int per = (k + 15) / 16;
+    for (int u = threadIdx.x; u < 16 * per; u += kThreads) {
+        const int r = u / per, c = (u - r * per) * 16;
+        uint32_t w[4];
+        __builtin_memcpy(w, __builtin_assume_aligned(lx + r * pitch + c, 16), 16);
+        if (first + r < rows) store_bytes<16>(codes + (first + r) * ldc + c, w, k - c);
+    }
+}
+
+// What a lane reads of a row in whole vectors; the one that ends the row, where it may not be read whole (the matrix's
+// last rows), comes by a load of its own: a short call is a straight run through its code, and lasts as long as that.
+template <class TX, int N, bool kWhole>
+__device__ __forceinline__ void load_row(v4i (&v)[N], const TX *p, int at, int step, int read, int k)
+{
+    constexpr int V = 16 / (int)sizeof(TX);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = v4i{0, 0, 0, 0};
+        if (at + i * step + V <= read) {
+            const LooseBytes<16>::type t = *reinterpret_cast<const LooseBytes<16>::type *>(p + at + i * step);
+            __builtin_memcpy(&v[i], &t, 16);
+        }
+    }
+    if (!kWhole && k % V && read == k) {
+        const int end = k / V * V;
+        const v4i e = load_elements<TX>(p + end, k - end);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (at + i * step == end) v[i] = e;
+    }
+}
+
+// Four rows of a workgroup's 16 a wavefront, each by all its lanes: codes at lx, scales at ls (k_int8_few).
+template <class TX, int IT, bool kWhole>
+__device__ __forceinline__ void code_four_rows(const TX *x, int64_t ldx, int64_t spare, int64_t first, int64_t rows, int k, int k64,
+                                               int8_t *lx, float *ls, float *scale)
+{
+    constexpr int V = RowVec<TX>::V;
     const int lane = threadIdx.x & 63, r0 = (threadIdx.x >> 6) * 4, pitch = k64 + 16;
-    const bool once = k <= IT * 64 * V;                    // the row fits the wavefront's registers
+    const bool once = IT == 1 || k <= IT * 64 * V;        // the row fits the wavefront's registers
     v4i raw[4][IT];
     uint32_t m[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            const int c = (i * 64 + lane) * V;
-            raw[r][i] = load_elements<TX, kWhole>(x + (first + r0 + r) * ldx + c, first + r0 + r < rows ? k - c : 0);
-        }
+        load_row<TX, IT, kWhole>(raw[r], x + (first + r0 + r) * ldx, lane * V, 64 * V, left_of(first + r0 + r, rows, spare, k, 0, V), k);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         float v[IT][V];
@@ -404,6 +444,7 @@ __device__ __forceinline__ void code_four_rows(const TX *x, int64_t ldx, const f
         for (int i = 0; i < IT; ++i) {
             TX t[V];
             __builtin_memcpy(t, &raw[r][i], 16);
+            if (!kWhole && k % V) clear_end(t, k - (i * 64 + lane) * V);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 v[i][j] = (float)t[j];
@@ -431,7 +472,6 @@ __device__ __forceinline__ void code_four_rows(const TX *x, int64_t ldx, const f
                 w[j / 4] = s.live ? q : 0u;
             }
             if (c < k64) __builtin_memcpy(__builtin_assume_aligned(lx + (r0 + r) * pitch + c, V), w, V);
-            if (codes && in) store_bytes<V>(codes + (first + r0 + r) * ldc + c, w, k - c);
         };
 #pragma unroll
         for (int i = 0; i < IT; ++i) put(v[i], (i * 64 + lane) * V);
@@ -443,25 +483,24 @@ __device__ __forceinline__ void code_four_rows(const TX *x, int64_t ldx, const f
             }
     }
 }
-template <bool kWhole>
 __device__ __forceinline__ void code_rows_given(const int8_t *x, int64_t ldx, const float *xs, int64_t first, int64_t rows, int k, int k64, int8_t *lx, float *ls)
 {
     const int per = k64 / 16;
     if (threadIdx.x < 16) ls[threadIdx.x] = first + threadIdx.x < rows ? xs[first + threadIdx.x] : 0.0f;
     for (int u = threadIdx.x; u < 16 * per; u += kThreads) {
         const int r = u / per, c = (u - r * per) * 16;
-        *reinterpret_cast<v4i *>(lx + r * (k64 + 16) + c) = load_elements<int8_t, kWhole>(x + (first + r) * ldx + c, first + r < rows ? k - c : 0);
+        *reinterpret_cast<v4i *>(lx + r * (k64 + 16) + c) = load_elements<int8_t>(x + (first + r) * ldx + c, first + r < rows ? k - c : 0);
     }
 }
 
 // Few rows: a workgroup takes 16 rows and 64 channels, 16 a wavefront.  The weights' loads are under way before the rows
 // are turned into codes (four rows a wavefront); nothing is read in turns, so a call lasts about three memory latencies.
-template <class TX, class T, bool kWhole>
-__global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx, const float *xs, int64_t rows, int k,
-                                                       const int8_t *w, int64_t ldw, const float *ws, int n, const float *bias,
+template <class TX, class T, int S, bool kWhole>             // kWhole: K is a multiple of 16
+__global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx, int64_t spare, const float *xs, int64_t rows, int k,
+                                                       const int8_t *w, int64_t ldw, int64_t spare_w, const float *ws, int n, const float *bias,
                                                        T *y, int64_t ldy, int8_t *codes, int64_t ldc, float *scale)
 {
-    constexpr int kAhead = 16;                             // steps of 64 whose weights are fetched first
+    constexpr int kAhead = 4 * S;                          // steps of 64 whose weights are fetched first
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];
     const int k64 = (k + 63) / 64 * 64, pitch = k64 + 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, quad = lane >> 4;
@@ -470,20 +509,21 @@ __global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx,
     int8_t *turn = lds + wave * 4096, *lx = lds + 4 * 4096;      // a wavefront's weights on their way to its operands: 4 steps
     float *ls = reinterpret_cast<float *>(lx + 16 * pitch);
     // four lanes take a row's 64 bytes of a step
-    const int8_t *wr = w + (int64_t)min(n0 + (lane >> 2), n - 1) * ldw;
-    const int part = (lane & 3) * 16;
+    const int wrow = min(n0 + (lane >> 2), n - 1), part = (lane & 3) * 16;
+    const int8_t *wr = w + (int64_t)wrow * ldw;
+    const int read = left_of(wrow, n, spare_w, k, 0, 16);      // weights beyond K meet codes that are zero
     v4i a[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) a[i] = load_elements<int8_t, kWhole>(wr + i * 64 + part, k - i * 64 - part);
+    load_row<int8_t, kAhead, kWhole>(a, wr, part, 64, read, k);
     const int64_t row = first + r16;
     const int c = n0 + quad * 4;
     float sc[4], bi[4] = {0.0f, 0.0f, 0.0f, 0.0f}, o[4];
     load_vec<float, 4>(sc, ws + c, n - c);
     if (bias) load_vec<float, 4>(bi, bias + c, n - c);
     if (blockIdx.y) codes = nullptr, scale = nullptr;
-    if constexpr (sizeof(TX) == 1) code_rows_given<kWhole>(x, ldx, xs, first, rows, k, k64, lx, ls);
-    else code_four_rows<TX, kWhole>(x, ldx, xs, first, rows, k, k64, lx, ls, codes, ldc, scale);
+    if constexpr (sizeof(TX) == 1) code_rows_given(x, ldx, xs, first, rows, k, k64, lx, ls);
+    else code_four_rows<TX, S, kWhole>(x, ldx, spare, first, rows, k, k64, lx, ls, scale);
     __syncthreads();
+    if (codes) codes_out(lx, pitch, first, rows, k, codes, ldc);
     v4i acc = {0, 0, 0, 0}, odd = {0, 0, 0, 0};            // two chains of sums: one would wait for itself
     const int8_t *at = lx + r16 * pitch + quad * 16;
     const auto four_steps = [&](const v4i *wv, int q) {
@@ -502,9 +542,9 @@ __global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx,
 #pragma unroll
     for (int i = 0; i < kAhead; i += 4)
         if (i * 64 < k64) four_steps(a + i, i * 64);
-    for (int q = kAhead * 64; q < k64; q += 256) {
+    for (int q = kAhead * 64; S > 1 && q < k64; q += 256) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = load_elements<int8_t, kWhole>(wr + q + i * 64 + part, k - q - i * 64 - part);
+        for (int i = 0; i < 4; ++i) a[i] = load_elements<int8_t>(wr + q + i * 64 + part, read - q - i * 64 - part);
         four_steps(a, q);
     }
     acc += odd;
@@ -635,7 +675,7 @@ struct AlongOperand {
         for (int n = 0; n < N; ++n) {
             const int u = threadIdx.x + n * kThreads, c = u % C * E;
             const T *p = base + min((int64_t)(u / C), na - 1 - a0) * ld + r + c;
-            v[n] = load_elements<T, false>(p, left - c);
+            v[n] = load_elements<T>(p, left - c);
         }
     }
     __device__ __forceinline__ void store(int8_t *lds) const
@@ -930,17 +970,20 @@ ProductPlan plan_product(int64_t rows, int k, int n, int x_type)
     ProductPlan p{};
     const int k64 = (k + 63) / 64 * 64, n64 = (n + 63) / 64 * 64, V = x_type == YH_INT8 ? 16 : x_type == YH_FLOAT32 ? 4 : 8;
     const size_t pitch = k64 + 16, wave = 16 * pitch + 16 * kOutPitch + 64;
-    // Up to two workgroups of 16 rows x 64 channels a compute unit: 338 rows, 1024 -> 512 take 8 us so, 12 us by tiles;
-    // 1352 rows, with four rounds of workgroups, 18 and 12.
+    // Up to two workgroups of 16 rows x 64 channels a compute unit: 828 rows, 1024 -> 512 take 8 us so, 12 us by tiles;
+    // 3000 rows, with six rounds of workgroups, 25 and 15.
     if ((rows + 15) / 16 * (n64 / 64) <= 512 && 16 * pitch + 64 <= 64 * 1024) {
         p.how = ProductPlan::kFew;
         p.lds = 4 * 4096 + 16 * pitch + 64;
         return p;
     }
     // Rows of up to 1024 bytes and weights that leave LDS room for eight wavefronts' rows; with longer rows (512 -> 128:
-    // 37 us by 16 rows, 31 by tiles) or with the weights in two halves the codes are better taken once, into memory.
+    // 37 us by 16 rows, 31 by tiles) or with the weights in two halves the codes are better taken once, into memory.  Every
+    // workgroup loads the weights first, which pays from four blocks of 16 rows a compute unit on (256 -> 128: 6000 rows 11.5
+    // us so, 8.4 by tiles; 24000 rows 15.9 both; 100000 rows 37.6 and 41.2), with 8 KiB of weights always (32 -> 64, 6000
+    // rows: 5.4 and 6.2 us).
     p.lds = n64 * (pitch + 8) + kRowWaves * wave;
-    if (k64 <= 64 * V && p.lds <= 160 * 1024) {
+    if (k64 <= 64 * V && p.lds <= 160 * 1024 && (rows >= 16384 || n64 * k64 <= 8192)) {
         p.how = ProductPlan::kRows;
         p.lanes = std::max(4, pow2_at_least((k64 / V + 3) / 4));
         return p;
@@ -950,14 +993,22 @@ ProductPlan plan_product(int64_t rows, int k, int n, int x_type)
 }
 
 template <class TX, class T, bool kWhole>
-void run_product(const ProductPlan &p, const TX *x, int64_t ldx, const float *xs, int64_t rows, int k, const int8_t *w, int64_t ldw, const float *ws,
-                 int n, const float *bias, T *y, int64_t ldy, int8_t *codes, int64_t ldc, float *scale, hipStream_t st)
+void run_few(const ProductPlan &p, const TX *x, int64_t ldx, const float *xs, int64_t rows, int k, const int8_t *w, int64_t ldw, const float *ws,
+             int n, const float *bias, T *y, int64_t ldy, int8_t *codes, int64_t ldc, float *scale, hipStream_t st)
 {
-    if (p.how == ProductPlan::kFew) {
-        k_int8_few<TX, T, kWhole><<<dim3((unsigned)((rows + 15) / 16), (n + 63) / 64), kThreads, p.lds, st>>>(x, ldx, xs, rows, k, w, ldw, ws, n, bias,
-                                                                                                              y, ldy, codes, ldc, scale);
-        return;
-    }
+    const int64_t spare = spare_rows(rows, ldx, 16 / (int)sizeof(TX));
+#define CALL(S)                                                                                                             \
+    k_int8_few<TX, T, S, kWhole><<<dim3((unsigned)((rows + 15) / 16), (n + 63) / 64), kThreads, p.lds, st>>>(               \
+        x, ldx, spare, xs, rows, k, w, ldw, spare_rows(n, ldw, 16), ws, n, bias, y, ldy, codes, ldc, scale)
+    if (k <= 256) CALL(1);
+    else CALL(4);
+#undef CALL
+}
+
+template <class TX, class T, bool kWhole>
+void run_rows(const ProductPlan &p, const TX *x, int64_t ldx, const float *xs, int64_t rows, int k, const int8_t *w, int64_t ldw, const float *ws,
+              int n, const float *bias, T *y, int64_t ldy, int8_t *codes, int64_t ldc, float *scale, hipStream_t st)
+{
     // as many workgroups as the compute units hold at once, or as there are rows for
     const int64_t held = 256 * (int64_t)(160 * 1024 / p.lds), asked = (rows + 16 * kRowWaves - 1) / (16 * kRowWaves);
     const unsigned blocks = (unsigned)std::min(held, asked);
@@ -985,8 +1036,8 @@ hipError_t launch_int8_product(const Rows &x, const float *x_scale, int64_t rows
             using T = decltype(t);
             const auto go = [&](auto tx) {
                 using TX = decltype(tx);
-                // 16-byte vectors of weights and of x that end with the row, or any length
-                const auto call = k % 16 == 0 ? run_product<TX, T, true> : run_product<TX, T, false>;
+                const auto call = p.how == ProductPlan::kRows ? (k % 16 ? run_rows<TX, T, false> : run_rows<TX, T, true>)
+                                                              : (k % 16 ? run_few<TX, T, false> : run_few<TX, T, true>);
                 call(p, static_cast<const TX *>(x.p), x.ld, x_scale, rows, k, w, ldw, w_scale, n, bias, static_cast<T *>(y), ldy, codes, ldc, scale, st);
             };
             if (x.type == YH_INT8) go((int8_t)0);
