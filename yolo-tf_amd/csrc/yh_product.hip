@@ -135,6 +135,10 @@ __device__ __forceinline__ void out_16x64(const v4i (&acc)[4], float s, const fl
     wave_sync();
 }
 
+// The tile form, from codes in memory: 43264 rows, 1536 -> 425 57 us (1.0 POP/s, half of what a large library product
+// reaches): a wavefront's 64 x 64 results ask LDS for as many cycles as the matrix instructions take, and the two do not
+// overlap (LDS alone 18 us, the matrix instructions alone 14; larger tiles, longer steps, loads further ahead and wave
+// priorities won nothing).
 template <class T, int BM, int BN>
 __global__ __launch_bounds__(kThreads) void k_int8_tile(const int8_t *x, int64_t ldx, const float *xs, int64_t rows, int k,
                                                         const int8_t *w, int64_t ldw, const float *ws, int n, const float *bias,
@@ -494,7 +498,9 @@ __device__ __forceinline__ void code_rows_given(const int8_t *x, int64_t ldx, co
 }
 
 // Few rows: a workgroup takes 16 rows and 64 channels, 16 a wavefront.  The weights' loads are under way before the rows
-// are turned into codes (four rows a wavefront); nothing is read in turns, so a call lasts about three memory latencies.
+// are turned into codes (four rows a wavefront); nothing is read in turns, so a call lasts about three memory latencies
+// and one pass through its code, which is why rows of up to 256 channels have a form of their own (S = 1; 300 rows,
+// 256 -> 128: 5.0 us, 6.0 with S = 4).  169 rows, 1024 -> 512: 6.6 us.
 template <class TX, class T, int S, bool kWhole>             // kWhole: K is a multiple of 16
 __global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx, int64_t spare, const float *xs, int64_t rows, int k,
                                                        const int8_t *w, int64_t ldw, int64_t spare_w, const float *ws, int n, const float *bias,
@@ -598,6 +604,9 @@ __device__ __forceinline__ void split8(const float (&x)[8], v8b (&out)[3])
 // Output indexes past the matrix's end read its last row or column again (what they give is not stored), so that a step
 // of 32 whole indexes of the sum asks nothing; offsets are 32 bits from a uniform base (pitches below 2^22: 128 rows of 4-byte elements).
 
+// Four wavefronts work on a tile together: a team.  Where a workgroup has several, each takes some of the sum's steps.
+__device__ __forceinline__ int team_thread() { return threadIdx.x & (kThreads - 1); }
+
 // Weight gradient: the sum runs down the rows of dy; a lane takes eight rows of a column straight into its operand, 16
 // lanes 16 neighbouring columns.
 template <class T>
@@ -609,8 +618,8 @@ struct DownOperand {
     int64_t ld;
     __device__ __forceinline__ void place(const T *p, int64_t pitch, int64_t a0, int64_t na)
     {
-        const int lane = threadIdx.x & 63;
-        const int64_t aw = min(a0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 16, na - 1);
+        const int lane = team_thread() & 63;
+        const int64_t aw = min(a0 + __builtin_amdgcn_readfirstlane(team_thread() >> 6) * 16, na - 1);
         base = p + aw;
         ld = pitch;
         off = (uint32_t)(((lane >> 4) * 8 * ld + min(aw + (lane & 15), na - 1) - aw) * sizeof(T));
@@ -627,7 +636,7 @@ struct DownOperand {
     }
     __device__ __forceinline__ void load_part(int64_t r, int left)
     {
-        const int k = ((threadIdx.x & 63) >> 4) * 8;
+        const int k = ((team_thread() & 63) >> 4) * 8;
         const uint32_t a = off - (uint32_t)(k * ld * sizeof(T));                  // the column alone, whatever the pitch
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = k + e < left ? (float)*(base + (r + k + e) * ld + a / sizeof(T)) : 0.0f;
@@ -659,7 +668,7 @@ struct AlongOperand {
         ld = pitch, a0 = first, na = rows;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int u = threadIdx.x + n * kThreads;
+            const int u = team_thread() + n * kThreads;
             off[n] = (uint32_t)((min((int64_t)(u / C), na - 1 - a0) * ld + u % C * E) * sizeof(T));
         }
     }
@@ -673,7 +682,7 @@ struct AlongOperand {
     {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int u = threadIdx.x + n * kThreads, c = u % C * E;
+            const int u = team_thread() + n * kThreads, c = u % C * E;
             const T *p = base + min((int64_t)(u / C), na - 1 - a0) * ld + r + c;
             v[n] = load_elements<T>(p, left - c);
         }
@@ -682,13 +691,13 @@ struct AlongOperand {
     {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int u = threadIdx.x + n * kThreads;
+            const int u = team_thread() + n * kThreads;
             __builtin_memcpy(__builtin_assume_aligned(lds + place_of(u / C, u % C), 16), &v[n], 16);
         }
     }
     __device__ __forceinline__ void fetch(const int8_t *lds, float (&x)[8]) const
     {
-        const int lane = threadIdx.x & 63, row = (threadIdx.x >> 6) * 16 + (lane & 15);
+        const int lane = team_thread() & 63, row = (team_thread() >> 6) * 16 + (lane & 15);
 #pragma unroll
         for (int h = 0; h < 8 / E; ++h) {
             T t[E];
@@ -709,13 +718,13 @@ struct TurnedTile {
     static constexpr int Q = BB / 4, N = (BB * 2 + kThreads - 1) / kThreads;
     uint32_t v[N][4], off[N];
     int shift;
-    __device__ __forceinline__ bool idle() const { return BB * 2 < kThreads && (int)threadIdx.x >= BB * 2; }
+    __device__ __forceinline__ bool idle() const { return BB * 2 < kThreads && team_thread() >= BB * 2; }
     __device__ __forceinline__ void place(int64_t ld, int left)          // left: columns from the tile's first on, at least 4
     {
-        const int b = threadIdx.x % Q * 4, c = min(b, left - 4);
+        const int b = team_thread() % Q * 4, c = min(b, left - 4);
         shift = min(b - c, 3) * 8;
 #pragma unroll
-        for (int n = 0; n < N; ++n) off[n] = (uint32_t)((threadIdx.x + n * kThreads) / Q * 4 * ld + c);
+        for (int n = 0; n < N; ++n) off[n] = (uint32_t)((team_thread() + n * kThreads) / Q * 4 * ld + c);
     }
     __device__ __forceinline__ void load_whole(const int8_t *base, int64_t ld)
     {
@@ -731,7 +740,7 @@ struct TurnedTile {
         if (idle()) return;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int b = threadIdx.x % Q * 4, r = (threadIdx.x + n * kThreads) / Q * 4;
+            const int b = team_thread() % Q * 4, r = (team_thread() + n * kThreads) / Q * 4;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 uint32_t w[1];
@@ -745,7 +754,7 @@ struct TurnedTile {
         if (idle()) return;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int q = threadIdx.x % Q, r = (threadIdx.x + n * kThreads) / Q;
+            const int q = team_thread() % Q, r = (team_thread() + n * kThreads) / Q;
             uint32_t x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = v[n][i] >> shift;
@@ -758,8 +767,8 @@ struct TurnedTile {
     }
 };
 
-// out[a, b] over 64 x 16 TB values from (a0, b0) on, the sum over [r0, r1) in steps of 32.
-template <class T, bool kDown, int TB, class TO, bool kSums>
+// out[a, b] over 64 x 16 TB values from (a0, b0) on, the sum over [r0, r1) in steps of 32, which the teams take in turn.
+template <class T, bool kDown, int TB, int kTeams, class TO, bool kSums>
 __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float *scale, const int8_t *q, int64_t ldq,
                                            int64_t a0, int64_t na, int b0, int nb, int64_t r0, int64_t r1,
                                            TO *out, int64_t ldo, float *sums)
@@ -767,8 +776,11 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
     typedef typename std::conditional<kDown, DownOperand<T>, AlongOperand<T>>::type Operand;
     constexpr int BB = 16 * TB, kB = BB * 64, kS = 128, kStage = Operand::kLds + kB + kS;
     constexpr int kPitch = BB * 4 + 16, kTurn = 4 * 16 * kPitch;      // the results' way out
-    __shared__ __attribute__((aligned(16))) int8_t lds[kTurn > 2 * kStage ? kTurn : 2 * kStage];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kTeam = kTurn > 2 * kStage ? kTurn : 2 * kStage;
+    __shared__ __attribute__((aligned(16))) int8_t all[kTeams * kTeam];
+    const int thread = team_thread(), team = kTeams > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads) : 0;
+    const int lane = thread & 63, wave = thread >> 6;
+    int8_t *lds = all + team * kTeam;
     v4f acc[TB];
 #pragma unroll
     for (int i = 0; i < TB; ++i) acc[i] = v4f{0, 0, 0, 0};
@@ -782,7 +794,7 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
     const auto store = [&](int8_t *stage) {
         fa.store(stage);
         tb.store(stage + Operand::kLds);
-        if (threadIdx.x < 32) reinterpret_cast<float *>(stage + Operand::kLds + kB)[threadIdx.x] = scale_v;
+        if (thread < 32) reinterpret_cast<float *>(stage + Operand::kLds + kB)[thread] = scale_v;
     };
     // the stage's float operand, scaled and split
     const auto split = [&](const int8_t *stage, v8b (&a)[3]) {
@@ -807,43 +819,63 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
                 for (int c = 0; c < 4; ++c) acc[i + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[c], a[p], acc[i + c], 0, 0, 0);
         }
     };
-    int64_t r = r0;
-    int at = 0;
     const int64_t whole = near ? r0 + (r1 - r0) / 32 * 32 : r0;      // up to here: steps that ask nothing, loaded one ahead
-    if (r < whole) {
+    constexpr int kRound = 32 * kTeams;
+    if (r0 < whole) {
         const auto load = [&](int64_t x) {
             fa.load_whole(x);
             tb.load_whole(pb + x * ldq, ldq);
-            if (threadIdx.x < 32) scale_v = scale[x + threadIdx.x];
+            if (thread < 32) scale_v = scale[x + thread];
         };
-        load(r);
-        store(lds);
+        int64_t r = r0 + team * 32;
+        int at = 0;
+        if (kTeams == 1 || r < whole) {
+            load(r);
+            store(lds);
+        }
         __syncthreads();
-        for (; r < whole; r += 32, at ^= 1) {
+        for (int64_t round = r0; round < whole; round += kRound, r += kRound, at ^= 1) {
             const int8_t *stage = lds + at * kStage;
             v8b a[3];
-            split(stage, a);
-            if (r + 32 < whole) load(r + 32);
-            multiply(stage, a);
-            // the other stage was read in the step before, and every wavefront has passed the barrier since
-            if (r + 32 < whole) store(lds + (at ^ 1) * kStage);
+            const bool on = kTeams == 1 || r < whole, more = r + kRound < whole;
+            if (on) split(stage, a);
+            if (more) load(r + kRound);
+            if (on) multiply(stage, a);
+            // the other stage was read in the round before, and every wavefront has passed the barrier since
+            if (more) store(lds + (at ^ 1) * kStage);
             __syncthreads();
         }
     }
-    for (; r < r1; r += 32) {
-        const int left = (int)min((int64_t)32, r1 - r);
+    for (int64_t round = whole; round < r1; round += kRound) {
+        const int64_t r = round + team * 32;
+        const int left = (int)max((int64_t)0, min((int64_t)32, r1 - r));
         fa.load_part(r, left);
         tb.load_part(pb + r * ldq, ldq, nb - b0, left);
-        if (threadIdx.x < 32) scale_v = (int)threadIdx.x < left ? scale[r + threadIdx.x] : 0.0f;
+        if (thread < 32) scale_v = thread < left ? scale[r + thread] : 0.0f;
         store(lds);
         __syncthreads();
-        v8b a[3];
-        split(lds, a);
-        multiply(lds, a);
+        if (left > 0) {
+            v8b a[3];
+            split(lds, a);
+            multiply(lds, a);
+        }
         __syncthreads();
     }
-    // A lane's four rows of LDS order j * BB / 4 + q are four
-    // neighbouring columns of the result; through LDS neighbouring lanes get neighbouring columns of a row.
+    if constexpr (kTeams > 1) {                                       // the teams' sums, added in order
+        static_assert(!kSums, "the rows' own sums stay with one team");
+        v4f *sums_of = reinterpret_cast<v4f *>(lds);
+#pragma unroll
+        for (int i = 0; i < TB; ++i)
+            if (team > 0) sums_of[i * kThreads + thread] = acc[i];
+        __syncthreads();
+        if (team > 0) return;
+#pragma unroll
+        for (int o = 1; o < kTeams; ++o)
+#pragma unroll
+            for (int i = 0; i < TB; ++i) acc[i] += reinterpret_cast<const v4f *>(all + o * kTeam)[i * kThreads + thread];
+    }
+    // A lane's four rows of LDS order j * BB / 4 + q are four neighbouring columns of the result; through LDS neighbouring
+    // lanes get neighbouring columns of a row.
     constexpr int H = TB / 4;
     int8_t *turn = lds + wave * 16 * kPitch;
     const int64_t first = a0 + wave * 16;
@@ -859,7 +891,7 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
             v4f o = {acc[h][e], acc[H + h][e], acc[2 * H + h][e], acc[3 * H + h][e]};
             *reinterpret_cast<v4f *>(turn + (lane & 15) * kPitch + (h * 16 + (lane >> 4) * 4 + e) * 16) = o;
         }
-    __syncthreads();
+    wave_sync();
 #pragma unroll
     for (int i = 0; i < TB; ++i) {
         const int u = i * 64 + lane, row = u / (BB / 4), b = u % (BB / 4) * 4;
@@ -870,7 +902,8 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
 }
 
 // Weight gradient: workgroup (tile of dw, piece of the rows).  The pieces' results are added by k_add_pieces in a fixed
-// order (no atomics: the same bits on every run).
+// order (no atomics: the same bits on every run).  1024 x 512 weights from 10816 rows: 40 us (34 GFLOP as three bfloat16
+// products, 0.86 PFLOP/s) and 6.7 us for the pieces; 128 x 64 from 692224 rows: 56 us (269 MB, 4.8 TB/s) and 8 us.
 template <class T, int TB>
 __global__ __launch_bounds__(kThreads, 2) void k_weight_grad(const T *dy, int64_t ldd, const int8_t *codes, int64_t ldc, const float *scale,
                                                              int64_t rows, int n, int k, int64_t rows_per_piece, int tiles_k, int tiles,
@@ -880,7 +913,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_weight_grad(const T *dy, int64_
     const int64_t piece = id / (uint32_t)tiles;
     const int tile = (int)(id % (uint32_t)tiles), a0 = tile / tiles_k * 64, b0 = tile % tiles_k * 16 * TB;
     const int64_t r0 = piece * rows_per_piece, r1 = min(rows, r0 + rows_per_piece);
-    split_tile<T, true, TB, float, true>(dy, ldd, scale, codes, ldc, a0, n, b0, k, r0, r1,
+    split_tile<T, true, TB, 1, float, true>(dy, ldd, scale, codes, ldc, a0, n, b0, k, r0, r1,
                                                 dw + piece * pitch, k, db && b0 == 0 ? db + piece * pitch : nullptr);
 }
 
@@ -911,12 +944,15 @@ __global__ __launch_bounds__(kThreads) void k_fill_zero(float *p, int64_t count)
     if (i < count) p[i] = 0.0f;
 }
 
-template <class T, int TB>
-__global__ __launch_bounds__(kThreads, 3) void k_input_grad(const T *dy, int64_t ldd, const int8_t *w, int64_t ldw, const float *ws,
+// Input gradient: workgroup (64 rows, 16 TB columns), the whole sum over the output channels.  Bound by the matrix
+// instructions and the vector instructions beside them: 43264 rows, 256 -> 512 in float32 41 us (34 GFLOP as three bfloat16
+// products: 0.83 PFLOP/s; the memory's share is 26 us), 21632 rows, 255 -> 128 12.5 us (2.7 TB/s).
+template <class T, int TB, int kTeams>
+__global__ __launch_bounds__(kThreads * kTeams, kTeams > 1 ? 1 : 3) void k_input_grad(const T *dy, int64_t ldd, const int8_t *w, int64_t ldw, const float *ws,
                                                             int64_t rows, int n, int k, int tiles_k, T *dx, int64_t lddx)
 {
     const uint32_t tile = (uint32_t)xcd_run(blockIdx.x, gridDim.x);
-    split_tile<T, false, TB, T, false>(dy, ldd, ws, w, ldw, (int64_t)(tile / (uint32_t)tiles_k) * 64, rows, (int)(tile % (uint32_t)tiles_k) * 16 * TB, k,
+    split_tile<T, false, TB, kTeams, T, false>(dy, ldd, ws, w, ldw, (int64_t)(tile / (uint32_t)tiles_k) * 64, rows, (int)(tile % (uint32_t)tiles_k) * 16 * TB, k,
                                                                    0, n, dx, lddx, nullptr);
 }
 
@@ -1060,7 +1096,8 @@ hipError_t launch_int8_product(const Rows &x, const float *x_scale, int64_t rows
             k_int8_tile<T, BM, BN><<<dim3((unsigned)((rows + BM - 1) / BM * tn)), kThreads, 0, st>>>(                       \
                 q, ldq, x_scale, rows, k, w, ldw, w_scale, n, bias, static_cast<T *>(y), ldy, tn);                          \
         } while (0)
-        // large tiles where they fill the card, small ones where there are few rows
+        // large tiles where they fill the card, small ones where there are few rows (1024 -> 512 in codes: 21632 rows 22.4 us
+        // large, 29.5 small; 5408 rows 13.3 and 11.5)
         if ((rows + 127) / 128 * ((n + 127) / 128) >= 256) CALL(128, 128);
         else CALL(64, 64);
 #undef CALL
@@ -1109,15 +1146,19 @@ hipError_t launch_input_grad(const Rows &dy, const int8_t *w, int64_t ldw, const
     (void)type;
     with_type(dy.type, [&](auto t) {
         using T = decltype(t);
-#define CALL(TB)                                                                                                            \
+#define CALL(TB, TEAMS)                                                                                                     \
         do {                                                                                                                \
             const int tk = (k + 16 * TB - 1) / (16 * TB);                                                                   \
-            k_input_grad<T, TB><<<dim3((unsigned)((rows + 63) / 64 * tk)), kThreads, 0, st>>>(                              \
+            k_input_grad<T, TB, TEAMS><<<dim3((unsigned)((rows + 63) / 64 * tk)), kThreads * TEAMS, 0, st>>>(               \
                 static_cast<const T *>(dy.p), dy.ld, w, ldw, w_scale, rows, n, k, tk, static_cast<T *>(dx), lddx);          \
         } while (0)
-        // (43264 rows, 256 -> 512: 40 us with 8, 45 with 16, 51 with 4); half as wide where that gives too few workgroups
-        if (k > 64 && (rows + 63) / 64 * ((k + 127) / 128) >= 256) CALL(8);
-        else CALL(4);
+        // Tiles of 64 x 128 (43264 rows, 256 -> 512: 40 us, 45 with 64 x 256, 51 with 64 x 64); half as wide where that gives
+        // too few workgroups, and with the sum over four teams where even so they are few and the sum is long (169 rows,
+        // 512 -> 1024, 48 workgroups: 8.2 us, 11.4 with one team; 32000 rows, 255 -> 60, 500 workgroups: 17.0 and 12.4; 2704
+        // rows, 128 -> 256, four steps: 5.6 and 5.3).
+        if (k > 64 && (rows + 63) / 64 * ((k + 127) / 128) >= 256) CALL(8, 1);
+        else if ((rows + 63) / 64 * ((k + 63) / 64) <= 256 && n > 160) CALL(4, 4);
+        else CALL(4, 1);
 #undef CALL
     });
     return hipGetLastError();
