@@ -395,14 +395,15 @@ int yh_loss_with_grad(const yh_head_config *cfg, const float *const *heads, cons
  *    atomics: every call can be captured into a graph, and gives the same bits on
  *    every run.
  *  - 0 <= rows < YH_MAX_ROWS, 1 <= channels <= YH_MAX_ROW_CHANNELS, and the product
- *    of any two of a call's sizes is below 2^38 (weights: below 2^31).
+ *    of any two of a call's sizes is below 2^36 (weights: below 2^31): what one launch
+ *    of the card takes.
  *
  * Codes of a row: scale = max|x| / 127 in float32, code = x * r rounded half to even
  * from the exact product, r = 127 / max|x| in float32; the value a code stands for
  * is code * scale.  A row whose largest magnitude is below 2^-110 is zero (scale 0).
  * A row that holds an infinity or a NaN has the scale NaN and codes 0: all that is
  * computed from it is NaN. */
-#define YH_MAX_ROWS (1 << 26)
+#define YH_MAX_ROWS ((1 << 26) - 64)
 #define YH_MAX_ROW_CHANNELS (1 << 16)
 
 /* codes [rows][k] int8, scale [rows], of x [rows][k]. */

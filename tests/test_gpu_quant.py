@@ -473,6 +473,52 @@ def test_offsets_beyond_32_bits(gpu):
     assert torch.equal(quant.input_grad(wide, *_layer(np.random.default_rng(1), 9, k, gpu)), quant.input_grad(x, *_layer(np.random.default_rng(1), 9, k, gpu)))
 
 
+@pytest.mark.parametrize('dtype', qc.TYPES)
+@pytest.mark.parametrize('m,k,n,gap', [(5, 7, 3, 1), (300, 37, 21, 9), (4500, 129, 130, 3), (40000, 30, 5, 2), (3000, 515, 70, 6), (60, 2051, 9, 5)])
+def test_what_lies_between_the_rows_has_no_effect(gpu, m, k, n, gap, dtype):
+    """Vectors may run over a row's end: the same bits whether NaN and whole codes lie there or the next row."""
+    rng = np.random.default_rng(38)
+
+    def apart(v):
+        wide = torch.full((v.shape[0], v.shape[1] + gap), 127 if v.dtype == torch.int8 else float('nan'), dtype=v.dtype, device=gpu)
+        wide[:, :v.shape[1]] = v
+        return wide[:, :v.shape[1]]
+
+    x, dy = _randn(rng, m, k).to(dtype).to(gpu), _randn(rng, m, n).to(dtype).to(gpu)
+    w, ws = _layer(rng, k, n, gpu)
+    q, s = (v.contiguous() for v in quant.quantize_rows(x))
+    w = w.contiguous()
+    for got, want in ((quant.quantize_rows(apart(x)), (q, s)),
+                      ((quant.dequantize_rows(apart(q), s),), (quant.dequantize_rows(q, s),)),
+                      (quant.matmul_int8(apart(x), apart(w), ws, want_codes=True), (quant.matmul_int8(x, w, ws), q, s)),
+                      ((quant.matmul_int8(apart(q), apart(w), ws, x_scale=s),), (quant.matmul_int8(q, w, ws, x_scale=s),)),
+                      (quant.weight_grad(apart(dy), apart(q), s, want_bias=True), quant.weight_grad(dy, q, s, want_bias=True)),
+                      ((quant.input_grad(apart(dy), apart(w), ws),), (quant.input_grad(dy, w, ws),))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    gamma, beta = (1 + 0.1 * _randn(rng, k)).to(gpu), (0.1 * _randn(rng, k)).to(gpu)
+    res = x.flip(0).contiguous()
+    a, kept = quant.norm_act(apart(x), gamma, beta, 1e-3, 0.1, residual=apart(res))
+    b, same = quant.norm_act(x, gamma, beta, 1e-3, 0.1, residual=res)
+    assert torch.equal(a, b) and torch.equal(kept.kept, same.kept) and torch.equal(kept.scale, same.scale)
+    da = _randn(rng, m, k).to(dtype).to(gpu)
+    assert all(torch.equal(g, h) for g, h in zip(quant.norm_act_backward(apart(da), kept), quant.norm_act_backward(da, same)))
+
+
+@pytest.mark.parametrize('dtype', qc.TYPES)
+@pytest.mark.parametrize('m,n,k', [(1, 161, 1), (70, 1122, 13), (169, 512, 200), (130, 300, 3), (64, 193, 64)])
+def test_input_grad_of_few_tiles(gpu, m, n, k, dtype):
+    """Long sums taken by several teams: against 64 bits, the terms within the float32 sum's bound."""
+    rng = np.random.default_rng(39)
+    w, ws = _layer(rng, k, n, gpu)
+    dy = _randn(rng, m, n).to(dtype)
+    got = quant.input_grad(dy.to(gpu), w, ws).double().cpu()
+    values = w.double().cpu() * ws.double().cpu()[:, None]
+    want, size = dy.double() @ values, dy.double().abs() @ values.abs()
+    # a term: one rounding of dy * w_scale; the sum: n + 3 additions of three pieces a term; the result's own rounding
+    bound = size * (3 * n + 8) * 2.0 ** -24 + want.abs() * (torch.finfo(dtype).eps / 2)
+    assert bool(((got - want).abs() <= bound + 1e-30).all())
+
+
 def test_pitches_beyond_the_short_offsets(gpu):
     """Rows 2^22 elements apart and more take the loads with 64-bit offsets."""
     rng = np.random.default_rng(34)

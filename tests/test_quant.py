@@ -99,7 +99,8 @@ def test_refusals_of_the_products():
     _refused(m(size=5000 * 5000 - 1, **wide), wsp, 'workspace')
     _refused(m(work=0x5008, size=1 << 30, **wide), ali, 'workspace')
     _refused(m(k=1 << 16, n=1 << 16), lim, 'weights')
-    _refused(m(rows=(1 << 26) - 1, k=1 << 15), lim, '2^38')
+    _refused(m(rows=(1 << 26) - 65, k=1 << 15), lim, '2^36')
+    _refused(m(rows=1 << 20, n=1 << 16), lim, '2^36')
     assert m(rows=0) == _abi.YH_OK
 
     def wg(dy=OK[0], t=F32, ld=5, c=OK[1], ldc=8, s=OK[2], rows=100000, n=5, k=8, dw=OK[3], db=OK[4], work=OK[5], size=1 << 30):

@@ -14,7 +14,7 @@ YH_STATUS_CANDIDATE_OVERFLOW = 1
 YH_STATUS_COUNT_SHIFT = 8
 YH_STATIC_SCRATCH_BYTES = 8 << 20
 
-YH_MAX_ROWS = 1 << 26
+YH_MAX_ROWS = (1 << 26) - 64
 YH_MAX_ROW_CHANNELS = 1 << 16
 YH_FLOAT32, YH_BFLOAT16, YH_FLOAT16, YH_INT8 = 0, 1, 2, 3
 

@@ -21,7 +21,7 @@ int check_sizes(int64_t rows, int32_t a, int32_t b)
     if (rows >= YH_MAX_ROWS) return yh::report(YH_ERR_LIMIT, "rows %lld is not below %d", (long long)rows, YH_MAX_ROWS);
     if (a > YH_MAX_ROW_CHANNELS || b > YH_MAX_ROW_CHANNELS)
         return yh::report(YH_ERR_LIMIT, "%d channels exceed %d", std::max(a, b), YH_MAX_ROW_CHANNELS);
-    if (rows * std::max(a, b) >= (int64_t)1 << 38) return yh::report(YH_ERR_LIMIT, "rows * channels is not below 2^38");
+    if (rows * std::max(a, b) >= (int64_t)1 << 36) return yh::report(YH_ERR_LIMIT, "rows * channels is not below 2^36");
     if ((int64_t)a * b >= (int64_t)1 << 31) return yh::report(YH_ERR_LIMIT, "%d x %d weights are not below 2^31", a, b);
     return YH_OK;
 }
