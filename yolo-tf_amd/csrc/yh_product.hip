@@ -342,8 +342,8 @@ struct CodeRows<int8_t, G, kWhole> {                     // codes already
 
 // Many rows, weights that fit: a workgroup keeps all weights in LDS for good and its eight wavefronts, which have nothing
 // more to say to each other, take blocks of 16 rows in turn, the next block's loads under this block's arithmetic.  Bound
-// by memory: 173056 rows, 256 -> 128 in float32 move 266 MB in 59 us (4.5 TB/s), 692224 rows, 128 -> 64 532 MB in 110 us
-// (4.8 TB/s); through codes in memory they take 77 and 179 us.
+// by memory: 173056 rows, 256 -> 128 in float32 move 266 MB in 56 us (4.8 TB/s), 692224 rows, 128 -> 64 532 MB in 108 us
+// (4.9 TB/s); through codes in memory they take 77 and 179 us.
 constexpr int kRowWaves = 8;
 
 template <class TX, class T, int G, bool kWhole>
@@ -945,8 +945,8 @@ __global__ __launch_bounds__(kThreads) void k_fill_zero(float *p, int64_t count)
 }
 
 // Input gradient: workgroup (64 rows, 16 TB columns), the whole sum over the output channels.  Bound by the matrix
-// instructions and the vector instructions beside them: 43264 rows, 256 -> 512 in float32 41 us (34 GFLOP as three bfloat16
-// products: 0.83 PFLOP/s; the memory's share is 26 us), 21632 rows, 255 -> 128 12.5 us (2.7 TB/s).
+// instructions and the vector instructions beside them: 43264 rows, 256 -> 512 in float32 42 us (34 GFLOP as three bfloat16
+// products: 0.81 PFLOP/s; the memory's share is 26 us), 21632 rows, 255 -> 128 12.5 us (2.7 TB/s).
 template <class T, int TB, int kTeams>
 __global__ __launch_bounds__(kThreads * kTeams, kTeams > 1 ? 1 : 3) void k_input_grad(const T *dy, int64_t ldd, const int8_t *w, int64_t ldw, const float *ws,
                                                             int64_t rows, int n, int k, int tiles_k, T *dx, int64_t lddx)

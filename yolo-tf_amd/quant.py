@@ -285,7 +285,8 @@ def norm_act(z, gamma, beta, eps, slope, residual=None, running=None, momentum=0
 
 
 def norm_act_backward(da, kept):
-    """(dz, dgamma [C], dbeta [C]) of norm_act from a's gradient and the NormKept; the residual's gradient is da."""
+    """(dz, dgamma [C], dbeta [C]) of norm_act from a's gradient and the NormKept (which reads gamma as it is now); the
+    residual's gradient is da."""
     dev = _device_of(da, 'da')
     kind = _float_type(da.dtype, 'da')
     if not kept.pitch:
