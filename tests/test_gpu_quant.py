@@ -121,7 +121,10 @@ def test_nothing_behind_a_row_or_the_last_row_is_written(gpu, m, k, n, pitch):
 PRODUCTS = [(1, 1, 1), (1, 1024, 255), (2, 77, 3), (5, 16, 64), (16, 65, 17), (40, 64, 32), (129, 255, 130), (300, 129, 257),
             (169, 1024, 512), (2000, 48, 27), (6000, 256, 640), (8, 6000, 20),
             # weights kept in LDS: one to sixteen lanes a row, whole and ragged rows; large tiles with a ragged end
-            (9000, 20, 16), (5000, 100, 130), (4500, 129, 200), (4500, 256, 70), (8200, 300, 64), (12000, 300, 520), (17000, 512, 256)]
+            (9000, 20, 16), (5000, 100, 130), (4500, 129, 200), (4500, 256, 70), (8200, 300, 64), (12000, 300, 520), (17000, 512, 256),
+            (16500, 100, 130), (20001, 255, 100), (16390, 256, 70), (16385, 300, 64),
+            # matrices and last tiles of fewer than four columns
+            (700, 1, 90), (701, 2, 90), (702, 3, 40), (500, 130, 66), (400, 258, 70)]
 
 
 def _layer(rng, k, n, dev):

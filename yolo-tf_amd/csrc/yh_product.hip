@@ -712,17 +712,20 @@ struct AlongOperand {
 // for the four wavefronts.  A unit is four columns x four rows of the sum; the lanes of a row of units read neighbouring
 // words.  Column 4 q + j of the tile becomes LDS row j * BB / 4 + q: the lanes that write column j of their units then
 // write neighbouring rows.  The last columns' unit starts where four are left and shifts them down; units past the end
-// read the last ones.
+// read the last ones.  Of a matrix of fewer than four columns a word runs over into the next row, which its last rows
+// (those from `spare` on) do not have.
 template <int BB>
 struct TurnedTile {
     static constexpr int Q = BB / 4, N = (BB * 2 + kThreads - 1) / kThreads;
     uint32_t v[N][4], off[N];
     int shift;
     __device__ __forceinline__ bool idle() const { return BB * 2 < kThreads && team_thread() >= BB * 2; }
-    __device__ __forceinline__ void place(int64_t ld, int left)          // left: columns from the tile's first on, at least 4
+    // The tile's first column in a matrix of nb, and where the whole words' base column is: `before` columns ahead of it.
+    __device__ __forceinline__ void place(int64_t ld, int b0, int nb, int &before)
     {
-        const int b = team_thread() % Q * 4, c = min(b, left - 4);
-        shift = min(b - c, 3) * 8;
+        const int last = max(nb - 4, 0), base = min(b0, last), b = b0 + team_thread() % Q * 4, c = min(b, last) - base;
+        before = b0 - base;
+        shift = min(b - base - c, 3) * 8;
 #pragma unroll
         for (int n = 0; n < N; ++n) off[n] = (uint32_t)((team_thread() + n * kThreads) / Q * 4 * ld + c);
     }
@@ -770,7 +773,7 @@ struct TurnedTile {
 // out[a, b] over 64 x 16 TB values from (a0, b0) on, the sum over [r0, r1) in steps of 32, which the teams take in turn.
 template <class T, bool kDown, int TB, int kTeams, class TO, bool kSums>
 __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float *scale, const int8_t *q, int64_t ldq,
-                                           int64_t a0, int64_t na, int b0, int nb, int64_t r0, int64_t r1,
+                                           int64_t spare, int64_t a0, int64_t na, int b0, int nb, int64_t r0, int64_t r1,
                                            TO *out, int64_t ldo, float *sums)
 {
     typedef typename std::conditional<kDown, DownOperand<T>, AlongOperand<T>>::type Operand;
@@ -788,9 +791,10 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
     TurnedTile<BB> tb;
     float scale_v = 0.0f, col = 0.0f;
     fa.place(dy, ldd, a0, na);
-    tb.place(ldq, max(4, nb - b0));
+    int before;
+    tb.place(ldq, b0, nb, before);
     const int8_t *pb = q + b0;
-    const bool near = nb - b0 >= 4 && ldd < (1 << 22) && ldq < (1 << 22);
+    const bool near = ldd < (1 << 22) && ldq < (1 << 22);
     const auto store = [&](int8_t *stage) {
         fa.store(stage);
         tb.store(stage + Operand::kLds);
@@ -819,12 +823,13 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
                 for (int c = 0; c < 4; ++c) acc[i + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[c], a[p], acc[i + c], 0, 0, 0);
         }
     };
-    const int64_t whole = near ? r0 + (r1 - r0) / 32 * 32 : r0;      // up to here: steps that ask nothing, loaded one ahead
+    // up to here: steps that ask nothing, loaded one ahead
+    const int64_t whole = near ? r0 + max((int64_t)0, (nb < 4 ? min(r1, spare) : r1) - r0) / 32 * 32 : r0;
     constexpr int kRound = 32 * kTeams;
     if (r0 < whole) {
         const auto load = [&](int64_t x) {
             fa.load_whole(x);
-            tb.load_whole(pb + x * ldq, ldq);
+            tb.load_whole(pb - before + x * ldq, ldq);
             if (thread < 32) scale_v = scale[x + thread];
         };
         int64_t r = r0 + team * 32;
@@ -906,14 +911,14 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
 // products, 0.86 PFLOP/s) and 6.7 us for the pieces; 128 x 64 from 692224 rows: 56 us (269 MB, 4.8 TB/s) and 8 us.
 template <class T, int TB>
 __global__ __launch_bounds__(kThreads, 2) void k_weight_grad(const T *dy, int64_t ldd, const int8_t *codes, int64_t ldc, const float *scale,
-                                                             int64_t rows, int n, int k, int64_t rows_per_piece, int tiles_k, int tiles,
+                                                             int64_t spare, int64_t rows, int n, int k, int64_t rows_per_piece, int tiles_k, int tiles,
                                                              float *dw, float *db, int64_t pitch)
 {
     const uint32_t id = (uint32_t)xcd_run(blockIdx.x, gridDim.x);
     const int64_t piece = id / (uint32_t)tiles;
     const int tile = (int)(id % (uint32_t)tiles), a0 = tile / tiles_k * 64, b0 = tile % tiles_k * 16 * TB;
     const int64_t r0 = piece * rows_per_piece, r1 = min(rows, r0 + rows_per_piece);
-    split_tile<T, true, TB, 1, float, true>(dy, ldd, scale, codes, ldc, a0, n, b0, k, r0, r1,
+    split_tile<T, true, TB, 1, float, true>(dy, ldd, scale, codes, ldc, spare, a0, n, b0, k, r0, r1,
                                                 dw + piece * pitch, k, db && b0 == 0 ? db + piece * pitch : nullptr);
 }
 
@@ -949,10 +954,10 @@ __global__ __launch_bounds__(kThreads) void k_fill_zero(float *p, int64_t count)
 // products: 0.81 PFLOP/s; the memory's share is 26 us), 21632 rows, 255 -> 128 12.5 us (2.7 TB/s).
 template <class T, int TB, int kTeams>
 __global__ __launch_bounds__(kThreads * kTeams, kTeams > 1 ? 1 : 3) void k_input_grad(const T *dy, int64_t ldd, const int8_t *w, int64_t ldw, const float *ws,
-                                                            int64_t rows, int n, int k, int tiles_k, T *dx, int64_t lddx)
+                                                            int64_t spare, int64_t rows, int n, int k, int tiles_k, T *dx, int64_t lddx)
 {
     const uint32_t tile = (uint32_t)xcd_run(blockIdx.x, gridDim.x);
-    split_tile<T, false, TB, kTeams, T, false>(dy, ldd, ws, w, ldw, (int64_t)(tile / (uint32_t)tiles_k) * 64, rows, (int)(tile % (uint32_t)tiles_k) * 16 * TB, k,
+    split_tile<T, false, TB, kTeams, T, false>(dy, ldd, ws, w, ldw, spare, (int64_t)(tile / (uint32_t)tiles_k) * 64, rows, (int)(tile % (uint32_t)tiles_k) * 16 * TB, k,
                                                                    0, n, dx, lddx, nullptr);
 }
 
@@ -1123,7 +1128,7 @@ hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, 
     with_type(dy.type, [&](auto t) {
         using T = decltype(t);
 #define CALL(TB) k_weight_grad<T, TB><<<dim3((unsigned)(p.tiles * p.pieces)), kThreads, 0, st>>>(                           \
-            static_cast<const T *>(dy.p), dy.ld, codes, ldc, scale, rows, n, k, p.rows_per_piece, p.tiles_k, p.tiles, pw, pb, pitch)
+            static_cast<const T *>(dy.p), dy.ld, codes, ldc, scale, spare_rows(rows, ldc, 4), rows, n, k, p.rows_per_piece, p.tiles_k, p.tiles, pw, pb, pitch)
         if (p.tb == 4) CALL(4);
         else if (p.tb == 8) CALL(8);
         else CALL(16);
@@ -1150,7 +1155,7 @@ hipError_t launch_input_grad(const Rows &dy, const int8_t *w, int64_t ldw, const
         do {                                                                                                                \
             const int tk = (k + 16 * TB - 1) / (16 * TB);                                                                   \
             k_input_grad<T, TB, TEAMS><<<dim3((unsigned)((rows + 63) / 64 * tk)), kThreads * TEAMS, 0, st>>>(               \
-                static_cast<const T *>(dy.p), dy.ld, w, ldw, w_scale, rows, n, k, tk, static_cast<T *>(dx), lddx);          \
+                static_cast<const T *>(dy.p), dy.ld, w, ldw, w_scale, spare_rows(n, ldw, 4), rows, n, k, tk, static_cast<T *>(dx), lddx);          \
         } while (0)
         // Tiles of 64 x 128 (43264 rows, 256 -> 512: 40 us, 45 with 64 x 256, 51 with 64 x 64); half as wide where that gives
         // too few workgroups, and with the sum over four teams where even so they are few and the sum is long (169 rows,
