@@ -176,7 +176,7 @@ def _grads(rng, m, n, dtype):
 
 
 @pytest.mark.parametrize('dtype', qc.TYPES)
-@pytest.mark.parametrize('m,k,n', PRODUCTS + [(0, 40, 30), (70000, 32, 64)])
+@pytest.mark.parametrize('m,k,n', PRODUCTS + [(0, 40, 30), (70000, 32, 64), (33001, 250, 512), (16640, 512, 512)])
 def test_weight_gradient(gpu, m, k, n, dtype):
     rng = np.random.default_rng(m + 7 * k + n)
     dy = _grads(rng, m, n, dtype)

@@ -969,18 +969,20 @@ void with_type(int32_t type, F f)
     else f((_Float16)0.0f);
 }
 
-// Tiles of 64 x 16 tb values: as wide as the result asks, so that the float operand is read and split as seldom as
-// possible (1024 x 512 weights from 10816 rows: 40 us with tb = 16, 45 us with 8).
+// Tiles of 64 x 16 tb values.  The widest reads and splits the float operand least often, which pays where each of 512
+// workgroups has 16 steps of 32 rows and more and the tiles are filled (1024 x 512 weights from 10816 rows: 48 us in all
+// with tb = 16, 53 with 8; from 2704 rows 512 x 256: 17.7 and 16.3; 384 x 255 from 43264 rows: 43.9 and 41.6).
 struct GradPlan { int tb, tiles_k, tiles, pieces; int64_t rows_per_piece; };
 GradPlan plan_weight_grad(int64_t rows, int n, int k)
 {
     GradPlan p;
-    p.tb = k <= 64 ? 4 : k <= 128 ? 8 : 16;
+    const int64_t steps = (rows + 31) / 32, wide = (k + 255) / 256;
+    p.tb = k <= 64 ? 4 : wide * 256 <= k + k / 4 && steps * ((n + 63) / 64) * wide >= 16 * 512 ? 16 : 8;
     p.tiles_k = (k + 16 * p.tb - 1) / (16 * p.tb);
     p.tiles = (n + 63) / 64 * p.tiles_k;
     // two workgroups a compute unit, each with at least four steps of 32 rows: more pieces cost more in k_add_pieces than
     // they win (692224 rows, 64 x 128: 64 us in all with 512 workgroups, 65 with 768, 69 with 1024)
-    const int64_t want = std::max(1, 512 / p.tiles), steps = (rows + 31) / 32;
+    const int64_t want = std::max(1, 512 / p.tiles);
     const int64_t pieces = std::max<int64_t>(1, std::min(want, (steps + 3) / 4));
     p.rows_per_piece = (steps + pieces - 1) / pieces * 32;
     p.pieces = (int)((rows + p.rows_per_piece - 1) / p.rows_per_piece);
