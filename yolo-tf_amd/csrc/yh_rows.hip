@@ -173,8 +173,8 @@ ReducePlan plan_reduce(int64_t rows, int cols, int V)
     const int cv = (cols + V - 1) / V;
     ReducePlan p;
     // Up to 1024 rows one workgroup takes all rows of a slab of four vectors (64 bytes a row) and finishes by itself: the
-    // launch that adds the partials costs more than what the spread over workgroups wins (forward and backward pass,
-    // 169 x 1024 in bfloat16: 18.9 us so, 24.2 with it; 1024 x 1024: 23.9 and 26.1; 4096 x 1024: 76.8 and 44.0).
+    // launch that adds the partials costs more than what the spread over workgroups wins (forward pass,
+    // 169 x 1024 in bfloat16: 9.7 us so, 12.0 with it; 1024 x 1024: 10.7 and 12.8; 4096 x 1024: 25.1 and 22.6).
     const bool alone = rows <= 1024;
     p.tx = std::min(alone ? 4 : 64, pow2_at_least(cv));
     p.ty = kThreads / p.tx;
@@ -258,6 +258,19 @@ struct NormGrads {
 
 // Statistics: one read of z.  346112 x 128 in float32 (177 MB): 45 us (3.9 TB/s), the adding of the partials 5 us; sums
 // in float32, loads one round ahead, half or twice the workgroups: 44 to 49 us.
+// The same, and a workgroup's own channels, from `first` on, in LDS.
+struct NormGradsHere {
+    NormGrads out;
+    float *b_here, *g_here;
+    int first;
+    __device__ __forceinline__ void finish(int c, double b, double g) const
+    {
+        out.finish(c, b, g);
+        b_here[c - first] = (float)b;
+        g_here[c - first] = (float)g;
+    }
+};
+
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int64_t spare, int TX, double *part,
                                                          NormStats<T> out)
@@ -532,6 +545,19 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply_long(const T *z, int64_
 __device__ __forceinline__ float kept_code(uint32_t w, int i) { return (float)((int8_t)(w >> (8 * i)) >> 1); }
 __device__ __forceinline__ bool kept_side(uint32_t w, int i) { return (w >> (8 * i)) & 1u; }
 
+// da -> dz, from a row's bytes and scale and the channels' factors.
+template <int V>
+__device__ __forceinline__ void input_grads(float (&v)[V], const uint32_t (&w)[V / 4], float s, float slope, const float (&g)[V],
+                                            const float (&cb)[V], const float (&cg)[V])
+{
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float du = kept_side(w[j / 4], j % 4) ? v[j] : slope * v[j];
+        const float xq = kept_code(w[j / 4], j % 4) * s;
+        v[j] = g[j] * (du - cb[j] - xq * cg[j]);
+    }
+}
+
 // Sums of the backward pass: da and the checkpoint in.  346112 x 128 in float32 (223 MB): 55 us (4.0 TB/s).
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
@@ -586,6 +612,59 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_
     reduce_pairs<V>(s1, s2, TX, cols, part, out);
 }
 
+// The whole backward pass for few rows: a workgroup holds its channels' rows, U a thread, and gives both the sums and the
+// input gradients.  169 x 1024 in bfloat16: 6.3 us, 9.3 in two
+// launches; 512 x 1024: 8.6 and 10.1.
+template <class T, int U>
+__global__ __launch_bounds__(kThreads) void k_norm_grad_few(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
+                                                            int64_t rows, int cols, float slope, int64_t spare, int TX, const float *gamma,
+                                                            const float *invstd, float *dgamma, float *dbeta, T *dz, int64_t ldz)
+{
+    constexpr int V = RowVec<T>::V;
+    __shared__ float sums[2][4 * V];
+    const int tx = threadIdx.x & (TX - 1), ty = threadIdx.x / TX, TY = kThreads / TX;
+    const int c = (blockIdx.y * TX + tx) * V;
+    float v[U][V], s[U], g[V], is[V], cb[V], cg[V];
+    uint32_t w[U][V / 4];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int64_t row = ty + i * TY;
+        const int read = left_of(row, rows, spare, cols, c, V);
+        load_vec<T, V>(v[i], da + row * ldd + c, read);
+        load_bytes<V>(w[i], kept + row * ldk + c, read);
+        s[i] = row < rows ? scale[row] : 0.0f;
+    }
+    load_vec<float, V>(g, gamma + c, cols - c);
+    load_vec<float, V>(is, invstd + c, cols - c);
+    double s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        s1[j] = s2[j] = 0.0;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {                // rows past the end are zeros
+            const float du = kept_side(w[i][j / 4], j % 4) ? v[i][j] : slope * v[i][j];
+            const float xq = kept_code(w[i][j / 4], j % 4) * s[i];
+            s1[j] += (double)du;
+            s2[j] = __builtin_fma((double)du, (double)xq, s2[j]);
+        }
+    }
+    reduce_pairs<V>(s1, s2, TX, cols, nullptr, NormGradsHere{{dgamma, dbeta}, sums[0], sums[1], (int)blockIdx.y * TX * V});
+    __syncthreads();
+    const float per_row = 1.0f / (float)rows;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        g[j] *= is[j];
+        cb[j] = sums[0][tx * V + j] * per_row;
+        cg[j] = sums[1][tx * V + j] * per_row;
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int64_t row = ty + i * TY;
+        input_grads<V>(v[i], w[i], s[i], slope, g, cb, cg);
+        if (row < rows) store_vec<T, V>(dz + row * ldz + c, v[i], cols - c);
+    }
+}
+
 __global__ __launch_bounds__(kThreads) void k_norm_grad_finish(const double *part, int blocks, int cols, int lanes, NormGrads out)
 {
     const int per = kThreads / lanes, c = min((int)blockIdx.x * per + (int)threadIdx.x / lanes, cols - 1), at = threadIdx.x & (lanes - 1);
@@ -636,12 +715,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int c = c0 + (i * lanes + sub) * V;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float du = kept_side(w[i][j / 4], j % 4) ? v[i][j] : slope * v[i][j];
-                const float xq = kept_code(w[i][j / 4], j % 4) * s;
-                v[i][j] = g[i][j] * (du - cb[i][j] - xq * cg[i][j]);
-            }
+            input_grads<V>(v[i], w[i], s, slope, g[i], cb[i], cg[i]);
             store_vec<T, V>(dz + row * ldz + c, v[i], cols - c);
         }
     }
@@ -765,8 +839,17 @@ hipError_t launch_norm_backward(const Rows &da, int64_t rows, int32_t cols, cons
         using T = decltype(t);
         const T *p = static_cast<const T *>(da.p);
         const ReducePlan d = plan_reduce(rows, cols, RowVec<T>::V);
-        const NormGrads out{dgamma, dbeta};
         const int64_t spare = std::min(spare_rows(rows, da.ld, RowVec<T>::V), spare_rows(rows, ldk, RowVec<T>::V));
+        // up to eight rows a thread in registers, where four vectors a row and no more are one workgroup's
+        if (d.tx <= 4 && rows <= 8 * d.ty) {
+#define CALL(U) k_norm_grad_few<T, U><<<dim3(1, d.slabs), kThreads, 0, st>>>(p, da.ld, kept, ldk, scale, rows, cols, slope, spare, d.tx, gamma, \
+                                                                            invstd, dgamma, dbeta, static_cast<T *>(dz), lddz)
+            if (rows <= 4 * d.ty) CALL(4);
+            else CALL(8);
+#undef CALL
+            return;
+        }
+        const NormGrads out{dgamma, dbeta};
         k_norm_grad_sums<T><<<dim3(d.blocks, d.slabs), kThreads, 0, st>>>(p, da.ld, kept, ldk, scale, rows, cols, slope, spare, d.tx, part, out);
         const int lanes = d.blocks > 64 ? kThreads : 64;
         if (d.blocks > 1)
