@@ -223,6 +223,55 @@ def test_a_step_under_autocast(gpu):
         assert float((a - b).norm() / b.norm()) < 0.05
 
 
+def _pointwise_layer(gpu):
+    torch.manual_seed(21)
+    layer = _layer(64, 48, 1, 1, True, 'int8', 'int8', gpu)
+    x = torch.randn(2, 64, 13, 13, device=gpu).contiguous(memory_format=torch.channels_last).requires_grad_()
+    res = torch.randn(2, 48, 13, 13, device=gpu).contiguous(memory_format=torch.channels_last)
+    da = torch.randn(2, 48, 13, 13, device=gpu).contiguous(memory_format=torch.channels_last)
+    return layer, x, res, da
+
+
+def test_a_graph_kept_for_a_second_backward_gives_the_same_again(gpu):
+    layer, x, res, da = _pointwise_layer(gpu)
+    leaves = [x] + list(layer.parameters())
+    out = layer(x, residual=res)
+    first = torch.autograd.grad(out, leaves, da, retain_graph=True)
+    second = torch.autograd.grad(out, leaves, da)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaves, da)
+
+
+def test_a_layer_captured_with_its_backward_replays_beside_eager_steps(gpu):
+    layer, x, res, da = _pointwise_layer(gpu)
+    leaves = [x] + list(layer.parameters())
+
+    def step():
+        out = layer(x, residual=res)
+        return [out.detach()] + list(torch.autograd.grad(out, leaves, da))
+
+    side = torch.cuda.Stream(gpu)
+    side.wait_stream(torch.cuda.current_stream(gpu))
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream(gpu).wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in range(4):
+        torch.manual_seed(100 + seed)
+        with torch.no_grad():
+            x.copy_(torch.randn_like(x))
+            da.copy_(torch.randn_like(da))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [g.clone() for g in got]
+        assert all(torch.equal(a, b) for a, b in zip(replayed, step()))
+
+
 def test_options_are_checked():
     with pytest.raises(ValueError, match='pointwise'):
         bb.Darknet19Head(2, 1, pointwise='int4')

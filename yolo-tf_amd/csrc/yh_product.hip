@@ -135,12 +135,13 @@ __device__ __forceinline__ void out_16x64(const v4i (&acc)[4], float s, const fl
     wave_sync();
 }
 
-// The tile form, from codes in memory: 43264 rows, 1536 -> 425 57 us (1.0 POP/s, half of what a large library product
-// reaches): a wavefront's 64 x 64 results ask LDS for as many cycles as the matrix instructions take, and the two do not
-// overlap (LDS alone 18 us, the matrix instructions alone 14; larger tiles, longer steps, loads further ahead and wave
-// priorities won nothing).
+// The tile form, from codes in memory: 43264 rows, 1536 -> 425 56 us (1.0 POP/s, half of what a large library product
+// reaches), 21632 rows, 1024 -> 512 22.6 us.  A wavefront's 64 x 64 results ask LDS for as many cycles as the matrix
+// instructions take (counted over a launch: matrix instructions busy 25 % of the cycles, LDS 32 %).  Operands read a step
+// ahead win 3 to 9 % where few wavefronts share a compute unit (2704 rows, 1024 -> 512 7.6 us, 8.3 without); larger tiles,
+// longer steps, loads further ahead and wave priorities won nothing.  Three workgroups a compute unit: 168 registers.
 template <class T, int BM, int BN>
-__global__ __launch_bounds__(kThreads) void k_int8_tile(const int8_t *x, int64_t ldx, const float *xs, int64_t rows, int k,
+__global__ __launch_bounds__(kThreads, 3) void k_int8_tile(const int8_t *x, int64_t ldx, const float *xs, int64_t rows, int k,
                                                         const int8_t *w, int64_t ldw, const float *ws, int n, const float *bias,
                                                         T *y, int64_t ldy, int tiles_n)
 {
@@ -170,42 +171,60 @@ __global__ __launch_bounds__(kThreads) void k_int8_tile(const int8_t *x, int64_t
         tx.store(stage);
         tw.store(stage + BM * 64);
     };
-    const auto multiply = [&](const int8_t *sx) {
+    struct Parts { v4i a[TN], b[TM]; };
+    const auto read = [&](Parts &f, const int8_t *sx) {
         const int8_t *sw = sx + BM * 64;
-        v4i a[TN], b[TM];
 #pragma unroll
-        for (int i = 0; i < TN; ++i) a[i] = *reinterpret_cast<const v4i *>(sw + chunk_at(wn + i * 16 + r16, quad));
+        for (int i = 0; i < TN; ++i) f.a[i] = *reinterpret_cast<const v4i *>(sw + chunk_at(wn + i * 16 + r16, quad));
 #pragma unroll
-        for (int j = 0; j < TM; ++j) b[j] = *reinterpret_cast<const v4i *>(sx + chunk_at(wm + j * 16 + r16, quad));
+        for (int j = 0; j < TM; ++j) f.b[j] = *reinterpret_cast<const v4i *>(sx + chunk_at(wm + j * 16 + r16, quad));
+    };
+    const auto multiply = [&](const Parts &f) {
 #pragma unroll
         for (int j = 0; j < TM; ++j)
 #pragma unroll
-            for (int i = 0; i < TN; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], b[j], acc[j][i], 0, 0, 0);
+            for (int i = 0; i < TN; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.a[i], f.b[j], acc[j][i], 0, 0, 0);
     };
     const int whole = ldx < (1 << 22) && ldw < (1 << 22) ? k & ~63 : 0;
     if (whole) {
-        tx.load_whole(0);
-        tw.load_whole(0);
+        // a step's operands are read from LDS while the step before is multiplied, stored while the one before that is, and
+        // loaded one step earlier still
+        Parts f[2];
+        const auto fetch = [&](int q) {
+            if (q < whole) {
+                tx.load_whole(q);
+                tw.load_whole(q);
+            }
+        };
+        fetch(0);
         store(lds);
+        fetch(64);
         __syncthreads();
-    }
-    int at = 0;
-    for (int q = 0; q < whole; q += 64, at ^= 1) {
-        if (q + 64 < whole) {
-            tx.load_whole(q + 64);
-            tw.load_whole(q + 64);
+        read(f[0], lds);
+        if (64 < whole) store(lds + kStage);
+        fetch(128);
+        __syncthreads();
+        const auto step = [&](int q, const Parts &now, Parts &next, int8_t *here, int8_t *there) {
+            if (q + 64 < whole) read(next, there);
+            multiply(now);
+            // this stage was read in the step before, and every wavefront has passed the barrier since
+            if (q + 128 < whole) store(here);
+            fetch(q + 192);
+            __syncthreads();
+        };
+        for (int q = 0; q < whole; q += 128) {
+            step(q, f[0], f[1], lds, lds + kStage);
+            if (q + 64 < whole) step(q + 64, f[1], f[0], lds + kStage, lds);
         }
-        multiply(lds + at * kStage);
-        // the other stage was read in the step before, and every wavefront has passed the barrier since
-        if (q + 64 < whole) store(lds + (at ^ 1) * kStage);
-        __syncthreads();
     }
     for (int q = whole; q < k; q += 64) {
         tx.load_part(q, k);
         tw.load_part(q, k);
         store(lds);
         __syncthreads();
-        multiply(lds);
+        Parts f;
+        read(f, lds);
+        multiply(f);
         __syncthreads();
     }
 #pragma unroll
