@@ -431,8 +431,10 @@ int yh_matmul_int8(const void *x, int32_t x_dtype, int64_t ldx, const float *x_s
 /* Gradient of that product (or of any product whose input is kept as codes) with
  * respect to the weights and the bias:
  *   dw[c][k] = sum_m dy[m][c] * scale[m] * codes[m][k],  db[c] = sum_m dy[m][c]
- * dw [n][k] float32, adjacent rows; db [n] may be NULL.  The terms are exact to
- * float32 and the sums float32 within a piece of the rows, 64 bits over the pieces.
+ * dw [n][k] float32, adjacent rows; db [n] may be NULL.  dw's terms are exact to
+ * float32, its sums float32 within a piece of the rows and 64 bits over the pieces
+ * (512 pieces and tiles of 64 x 64 to 64 x 256 weights together: beyond 256 tiles the
+ * rows are one piece).  db is summed in 64 bits throughout and rounded once.
  * An infinity in dy counts as a NaN.  rows = 0 gives zeros. */
 int yh_weight_grad_workspace_bytes(int64_t rows, int32_t n, int32_t k, size_t *bytes);
 int yh_weight_grad(const void *dy, int32_t dtype, int64_t lddy, const int8_t *codes, int64_t ldc, const float *scale,

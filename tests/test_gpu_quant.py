@@ -617,3 +617,20 @@ def test_empty_batches(gpu):
     assert (dw == 0).all() and (db == 0).all() and dw.shape == (5, 32)
     with pytest.raises(Exception, match='no rows'):
         quant.norm_act(x, torch.ones(32, device=gpu), torch.ones(32, device=gpu), 1e-3, 0.1)
+
+
+@pytest.mark.parametrize('positive', [True, False])
+@pytest.mark.parametrize('dtype', qc.TYPES)
+@pytest.mark.parametrize('m,k,n', [(1, 1, 1), (500, 40, 66), (33001, 40, 3), (70001, 64, 64), (9000, 300, 130), (20011, 2100, 2000)])
+def test_bias_gradient_is_a_sum_in_64_bits(gpu, m, k, n, dtype, positive):
+    """One rounding to float32 of a sum in 64 bits, whatever the pieces of the rows (the last size is one piece of 626 steps);
+    values of one sign, whose errors would add up, and of both, whose sum is far below its terms."""
+    g = torch.Generator(device=gpu).manual_seed(m + k)
+    dy = torch.rand(m, n, generator=g, device=gpu) + 0.5 if positive else torch.randn(m, n, generator=g, device=gpu)
+    dy = dy.to(dtype)
+    codes = torch.randint(-127, 128, (m, k), generator=g, device=gpu, dtype=torch.int8)
+    scale = torch.rand(m, generator=g, device=gpu)
+    _, db = quant.weight_grad(dy, codes, scale, want_bias=True)
+    want, size = dy.double().sum(0), dy.double().abs().sum(0)
+    # half a step of float32, and m additions in 64 bits on either side
+    assert ((db.double() - want).abs() <= qc.U * want.abs() + 2 * m * 2.0 ** -53 * size).all()

@@ -790,10 +790,13 @@ struct TurnedTile {
 };
 
 // out[a, b] over 64 x 16 TB values from (a0, b0) on, the sum over [r0, r1) in steps of 32, which the teams take in turn.
+// kSums: the float operand's own sums over [r0, r1), in 64 bits, go to `piece` as they are or to `sums` rounded once
+// (nowhere if both are null).  Every tile adds them, beside its matrix instructions and without a branch: 1 % of a call
+// more than float32 sums took (left to the one tile that stores them 2 to 6 %, the branch keeps loads and sums apart).
 template <class T, bool kDown, int TB, int kTeams, class TO, bool kSums>
 __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float *scale, const int8_t *q, int64_t ldq,
                                            int64_t spare, int64_t a0, int64_t na, int b0, int nb, int64_t r0, int64_t r1,
-                                           TO *out, int64_t ldo, float *sums)
+                                           TO *out, int64_t ldo, double *piece, float *sums)
 {
     typedef typename std::conditional<kDown, DownOperand<T>, AlongOperand<T>>::type Operand;
     constexpr int BB = 16 * TB, kB = BB * 64, kS = 128, kStage = Operand::kLds + kB + kS;
@@ -808,7 +811,8 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
     for (int i = 0; i < TB; ++i) acc[i] = v4f{0, 0, 0, 0};
     Operand fa;
     TurnedTile<BB> tb;
-    float scale_v = 0.0f, col = 0.0f;
+    float scale_v = 0.0f;
+    double col = 0.0;
     fa.place(dy, ldd, a0, na);
     int before;
     tb.place(ldq, b0, nb, before);
@@ -820,16 +824,22 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
         if (thread < 32) reinterpret_cast<float *>(stage + Operand::kLds + kB)[thread] = scale_v;
     };
     // the stage's float operand, scaled and split
-    const auto split = [&](const int8_t *stage, v8b (&a)[3]) {
-        float x[8], s[8];
+    const auto split = [&](const int8_t *stage, v8b (&a)[3], float (&x)[8]) {
+        float s[8];
         fa.fetch(stage, x);
         __builtin_memcpy(s, __builtin_assume_aligned(stage + Operand::kLds + kB + (lane >> 4) * 32, 16), 32);
-        if (kSums) col += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        float t[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= s[e];
-        split8(x, a);
+        for (int e = 0; e < 8; ++e) t[e] = x[e] * s[e];
+        split8(t, a);
     };
-    const auto multiply = [&](const int8_t *stage, const v8b (&a)[3]) {
+    const auto multiply = [&](const int8_t *stage, const v8b (&a)[3], const float (&x)[8]) {
+        if constexpr (kSums) {
+            double d[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = (double)x[e];
+            col += ((d[0] + d[1]) + (d[2] + d[3])) + ((d[4] + d[5]) + (d[6] + d[7]));
+        }
         // four blocks of columns at a time: an accumulator comes round again after four instructions, not at once
 #pragma unroll
         for (int i = 0; i < TB; i += 4) {
@@ -861,10 +871,11 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
         for (int64_t round = r0; round < whole; round += kRound, r += kRound, at ^= 1) {
             const int8_t *stage = lds + at * kStage;
             v8b a[3];
+            float x[8];
             const bool on = kTeams == 1 || r < whole, more = r + kRound < whole;
-            if (on) split(stage, a);
+            if (on) split(stage, a, x);
             if (more) load(r + kRound);
-            if (on) multiply(stage, a);
+            if (on) multiply(stage, a, x);
             // the other stage was read in the round before, and every wavefront has passed the barrier since
             if (more) store(lds + (at ^ 1) * kStage);
             __syncthreads();
@@ -880,8 +891,9 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
         __syncthreads();
         if (left > 0) {
             v8b a[3];
-            split(lds, a);
-            multiply(lds, a);
+            float x[8];
+            split(lds, a, x);
+            multiply(lds, a, x);
         }
         __syncthreads();
     }
@@ -903,10 +915,13 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
     constexpr int H = TB / 4;
     int8_t *turn = lds + wave * 16 * kPitch;
     const int64_t first = a0 + wave * 16;
-    if (kSums && sums) {
+    if (kSums && (piece || sums)) {
         col += __shfl_xor(col, 16);
         col += __shfl_xor(col, 32);
-        if (lane < 16 && first + lane < na) sums[first + lane] = col;
+        if (lane < 16 && first + lane < na) {
+            if (piece) piece[first + lane] = col;
+            else sums[first + lane] = (float)col;
+        }
     }
 #pragma unroll
     for (int h = 0; h < H; ++h)
@@ -931,27 +946,32 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
 template <class T, int TB>
 __global__ __launch_bounds__(kThreads, 2) void k_weight_grad(const T *dy, int64_t ldd, const int8_t *codes, int64_t ldc, const float *scale,
                                                              int64_t spare, int64_t rows, int n, int k, int64_t rows_per_piece, int tiles_k, int tiles,
-                                                             float *dw, float *db, int64_t pitch)
+                                                             float *dw, float *db, double *db_pieces)
 {
     const uint32_t id = (uint32_t)xcd_run(blockIdx.x, gridDim.x);
     const int64_t piece = id / (uint32_t)tiles;
     const int tile = (int)(id % (uint32_t)tiles), a0 = tile / tiles_k * 64, b0 = tile % tiles_k * 16 * TB;
     const int64_t r0 = piece * rows_per_piece, r1 = min(rows, r0 + rows_per_piece);
-    split_tile<T, true, TB, 1, float, true>(dy, ldd, scale, codes, ldc, spare, a0, n, b0, k, r0, r1,
-                                                dw + piece * pitch, k, db && b0 == 0 ? db + piece * pitch : nullptr);
+    split_tile<T, true, TB, 1, float, true>(dy, ldd, scale, codes, ldc, spare, a0, n, b0, k, r0, r1, dw + piece * ((int64_t)n * k), k,
+                                            db_pieces && b0 == 0 ? db_pieces + piece * n : nullptr, db && b0 == 0 ? db : nullptr);
 }
 
-// out[i] = sum of part[p][i] over the pieces, in 64 bits; the first `cut` values are dw, the others db.  A workgroup takes
-// `wide` values; its 256 / wide groups of threads add pieces in turn, and their sums are added in order.
-__global__ __launch_bounds__(kThreads) void k_add_pieces(const float *part, int pieces, int64_t count, int64_t cut, int wide, float *dw, float *db)
+// Sums over the pieces in 64 bits: the first `cut` of `count` values are dw, from float32 pieces, the others db, from pieces
+// of 64 bits.  A workgroup takes `wide` values; its 256 / wide groups of threads add pieces in turn, and their sums are
+// added in order.
+__global__ __launch_bounds__(kThreads) void k_add_pieces(const float *dw_pieces, const double *db_pieces, int pieces, int64_t count, int64_t cut,
+                                                         int wide, float *dw, float *db)
 {
     __shared__ double buf[kThreads];
     const int col = threadIdx.x & (wide - 1), group = threadIdx.x / wide, groups = kThreads / wide;
-    const int64_t i = (int64_t)blockIdx.x * wide + col;
+    const int64_t i = (int64_t)(gridDim.x - 1 - blockIdx.x) * wide + col;      // db's few first, under dw's
     double s = 0.0;
-    if (i < count) {
+    if (i < cut) {
 #pragma unroll 8
-        for (int p = group; p < pieces; p += groups) s += (double)part[p * count + i];
+        for (int p = group; p < pieces; p += groups) s += (double)dw_pieces[p * cut + i];
+    } else if (i < count) {
+#pragma unroll 8
+        for (int p = group; p < pieces; p += groups) s += db_pieces[p * (count - cut) + i - cut];
     }
     buf[threadIdx.x] = s;
     __syncthreads();
@@ -977,7 +997,7 @@ __global__ __launch_bounds__(kThreads * kTeams, kTeams > 1 ? 1 : 3) void k_input
 {
     const uint32_t tile = (uint32_t)xcd_run(blockIdx.x, gridDim.x);
     split_tile<T, false, TB, kTeams, T, false>(dy, ldd, ws, w, ldw, spare, (int64_t)(tile / (uint32_t)tiles_k) * 64, rows, (int)(tile % (uint32_t)tiles_k) * 16 * TB, k,
-                                                                   0, n, dx, lddx, nullptr);
+                                                                   0, n, dx, lddx, nullptr, nullptr);
 }
 
 template <class F>
@@ -1131,7 +1151,12 @@ hipError_t launch_int8_product(const Rows &x, const float *x_scale, int64_t rows
     return hipGetLastError();
 }
 
-int weight_grad_chunks(int64_t rows, int32_t n, int32_t k) { return plan_weight_grad(rows, n, k).pieces; }
+size_t weight_grad_workspace(int64_t rows, int32_t n, int32_t k)
+{
+    if (rows == 0) return 0;
+    const GradPlan p = plan_weight_grad(rows, n, k);
+    return p.pieces > 1 ? (size_t)p.pieces * ((size_t)n * k * sizeof(float) + n * sizeof(double)) : 0;
+}
 
 hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, const float *scale, int64_t rows,
                               int32_t n, int32_t k, float *dw, float *db, void *workspace, hipStream_t st)
@@ -1143,13 +1168,13 @@ hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, 
         return hipGetLastError();
     }
     const GradPlan p = plan_weight_grad(rows, n, k);
-    float *pw = p.pieces > 1 ? static_cast<float *>(workspace) : dw;
-    float *pb = !db ? nullptr : p.pieces > 1 ? pw + count : db;
-    const int64_t pitch = db ? count + n : count;              // a piece: dw, then db
+    // in the workspace: db's pieces (64 bits), then dw's
+    double *pb = p.pieces > 1 && db ? static_cast<double *>(workspace) : nullptr;
+    float *pw = p.pieces > 1 ? reinterpret_cast<float *>(static_cast<double *>(workspace) + (int64_t)p.pieces * n) : dw;
     with_type(dy.type, [&](auto t) {
         using T = decltype(t);
 #define CALL(TB) k_weight_grad<T, TB><<<dim3((unsigned)(p.tiles * p.pieces)), kThreads, 0, st>>>(                           \
-            static_cast<const T *>(dy.p), dy.ld, codes, ldc, scale, spare_rows(rows, ldc, 4), rows, n, k, p.rows_per_piece, p.tiles_k, p.tiles, pw, pb, pitch)
+            static_cast<const T *>(dy.p), dy.ld, codes, ldc, scale, spare_rows(rows, ldc, 4), rows, n, k, p.rows_per_piece, p.tiles_k, p.tiles, pw, db, pb)
         if (p.tb == 4) CALL(4);
         else if (p.tb == 8) CALL(8);
         else CALL(16);
@@ -1159,9 +1184,10 @@ hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, 
         // A thread a value where that gives 512 workgroups (512 x 256 weights from 43264 rows, 64 pieces: 45.9 us in all, 47.9
         // with eight threads a value); otherwise several threads a value, down to 16 neighbouring values (64 bytes) a
         // workgroup (128 x 64 weights from 692224 rows, 512 pieces: 63 us, 81 with a thread a value).
+        const int64_t values = db ? count + n : count;
         int wide = kThreads;
-        while (wide > 16 && pitch / wide < 512 && kThreads / wide < p.pieces) wide /= 2;
-        k_add_pieces<<<dim3((unsigned)((pitch + wide - 1) / wide)), kThreads, 0, st>>>(pw, p.pieces, pitch, count, wide, dw, db);
+        while (wide > 16 && values / wide < 512 && kThreads / wide < p.pieces) wide /= 2;
+        k_add_pieces<<<dim3((unsigned)((values + wide - 1) / wide)), kThreads, 0, st>>>(pw, pb, p.pieces, values, count, wide, dw, db);
     }
     return hipGetLastError();
 }

@@ -38,7 +38,7 @@ hipError_t launch_int8_product(const Rows &x, const float *x_scale, int64_t rows
                                const int8_t *w, int64_t ldw, const float *w_scale, int32_t n, const float *bias,
                                void *y, int64_t ldy, int32_t type, int8_t *codes, int64_t ldc, float *scale, hipStream_t st);
 
-int weight_grad_chunks(int64_t rows, int32_t n, int32_t k);     // pieces the rows are cut into
+size_t weight_grad_workspace(int64_t rows, int32_t n, int32_t k);     // bytes
 hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, const float *scale, int64_t rows,
                               int32_t n, int32_t k, float *dw, float *db, void *workspace, hipStream_t st);
 hipError_t launch_input_grad(const Rows &dy, const int8_t *w, int64_t ldw, const float *w_scale, int64_t rows,

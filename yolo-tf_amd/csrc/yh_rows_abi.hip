@@ -140,8 +140,7 @@ int yh_weight_grad_workspace_bytes(int64_t rows, int32_t n, int32_t k, size_t *b
 {
     if (!bytes) return yh::report(YH_ERR_INVALID_ARG, "bytes is null");
     YH_TRY(check_sizes(rows, n, k));
-    const int pieces = rows > 0 ? yh::weight_grad_chunks(rows, n, k) : 1;
-    *bytes = pieces > 1 ? (size_t)pieces * ((size_t)n * k + n) * sizeof(float) : 0;
+    *bytes = yh::weight_grad_workspace(rows, n, k);
     return YH_OK;
 }
 
