@@ -634,3 +634,16 @@ def test_bias_gradient_is_a_sum_in_64_bits(gpu, m, k, n, dtype, positive):
     want, size = dy.double().sum(0), dy.double().abs().sum(0)
     # half a step of float32, and m additions in 64 bits on either side
     assert ((db.double() - want).abs() <= qc.U * want.abs() + 2 * m * 2.0 ** -53 * size).all()
+
+
+def test_the_backward_pass_reads_gamma_as_it_is_now(gpu):
+    """Twice the gamma, twice the input gradient, bit for bit; also where gamma's values are not adjacent."""
+    torch.manual_seed(41)
+    z, da, beta = torch.randn(300, 40, device=gpu), torch.randn(300, 40, device=gpu), torch.randn(40, device=gpu)
+    for gamma in (torch.randn(40, device=gpu), torch.randn(40, 2, device=gpu)[:, 1]):
+        _, kept = quant.norm_act(z, gamma, beta, 1e-3, 0.1)
+        first = quant.norm_act_backward(da, kept)
+        gamma.mul_(2)
+        second = quant.norm_act_backward(da, kept)
+        assert torch.equal(second[0], 2 * first[0])
+        assert torch.equal(second[1], first[1]) and torch.equal(second[2], first[2])

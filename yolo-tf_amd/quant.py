@@ -258,7 +258,7 @@ def norm_act(z, gamma, beta, eps, slope, residual=None, running=None, momentum=0
     dev = _device_of(z, 'z')
     kind = _float_type(z.dtype, 'z')
     zr, rows, c, ldz = _rows(z, 'z')
-    gamma, beta = _vector(gamma, c, dev, 'gamma'), _vector(beta, c, dev, 'beta')
+    gr, beta = _vector(gamma, c, dev, 'gamma'), _vector(beta, c, dev, 'beta')
     rr, ldr = None, 0
     if residual is not None:
         if not isinstance(residual, torch.Tensor) or residual.shape != z.shape or residual.dtype != z.dtype or residual.device != dev:
@@ -278,7 +278,7 @@ def norm_act(z, gamma, beta, eps, slope, residual=None, running=None, momentum=0
     at = store.data_ptr()
     ws, nbytes, keep = _scratch('yh_norm_act_workspace_bytes', z, rows, c, kind)
     _call(dev, _abi.load().yh_norm_act_forward, zr.data_ptr(), ldz, None if rr is None else rr.data_ptr(), ldr, kind, rows, c,
-          gamma.data_ptr(), beta.data_ptr(), float(eps), slope, a.data_ptr(), c,
+          gr.data_ptr(), beta.data_ptr(), float(eps), slope, a.data_ptr(), c,
           at if want_kept else None, pitch, at + rows * pitch if want_kept else None, at + head, at + head + 4 * c,
           None if rm is None else rm.data_ptr(), None if rv is None else rv.data_ptr(), float(momentum), ws, nbytes)
     return a, NormKept(store, shape, rows, pitch, gamma, slope)
