@@ -185,3 +185,22 @@ def test_the_plain_statement_of_the_codes():
     q, s = qc.rows_of(x)
     assert q.tolist() == [[0, 0, 0], [127, 2, -2], [127, 32, -127], [0, 0, 0], [0, 0, 0], [0, 0, 0]]
     assert s[:2].tolist() == [0, 1] and s[3] == 0 and np.isnan(s[4:]).all()
+
+
+def test_channel_counts_that_do_not_fit_a_call_are_refused(monkeypatch):
+    """2^32 + 5 channels would reach the library as 5."""
+    monkeypatch.setattr(quant, '_device_of', lambda x, what: x.device)            # tensors without memory
+    most = _abi.YH_MAX_ROW_CHANNELS
+    meta = lambda *shape, dtype=torch.float32: torch.empty(shape, device='meta', dtype=dtype)
+    codes = lambda *shape: meta(*shape, dtype=torch.int8)
+    for n in (most + 1, 2 ** 31, 2 ** 32 + 5):
+        g = meta(n)
+        for call in (lambda: quant.quantize_rows(meta(1, n)), lambda: quant.dequantize_rows(codes(1, n), meta(1)),
+                     lambda: quant.matmul_int8(meta(2, n), codes(3, n), meta(3)), lambda: quant.matmul_int8(meta(2, 4), codes(n, 4), g),
+                     lambda: quant.weight_grad(meta(2, n), codes(2, 4), meta(2)), lambda: quant.weight_grad(meta(2, 4), codes(2, n), meta(2)),
+                     lambda: quant.input_grad(meta(2, n), codes(n, 4), g), lambda: quant.input_grad(meta(2, 4), codes(4, n), meta(4)),
+                     lambda: quant.norm_act(meta(2, n), g, g, 1e-3, 0.1)):
+            with pytest.raises(_abi.YhError, match='channels exceed') as refusal:
+                call()
+            assert refusal.value.code == _abi.YH_ERR_LIMIT
+    assert quant._rows(meta(3, most), 'x')[1:] == (3, most, most)

@@ -49,12 +49,19 @@ def _float_type(dtype, what):
     return code
 
 
+def _check_channels(n, what):
+    """Refuses what the library would, before a count beyond 32 bits is cut to what fits its argument."""
+    if n > _abi.YH_MAX_ROW_CHANNELS:
+        raise _abi.YhError(_abi.YH_ERR_LIMIT, '%s: %d channels exceed %d' % (what, n, _abi.YH_MAX_ROW_CHANNELS))
+
+
 def _rows(x, what):
     """x as [rows, channels] with adjacent channels: (tensor that owns the memory, rows, channels, elements between rows)."""
     shape = x.shape
     if not shape or shape[-1] < 1:
         raise ValueError('%s must be [..., channels] with at least one channel, got %s' % (what, tuple(shape)))
     cols = shape[-1]
+    _check_channels(cols, what)
     if x.is_contiguous():
         return x, x.numel() // cols, cols, cols
     x = x.detach()
@@ -152,6 +159,7 @@ def matmul_int8(x, w_codes, w_scale, bias=None, x_scale=None, out_dtype=None, wa
     wr, n, wk, ldw = _codes(w_codes, dev, 'w_codes')
     if w_codes.dim() != 2 or wk != k:
         raise ValueError('w_codes must be [N, %d], got %s' % (k, tuple(w_codes.shape)))
+    _check_channels(n, 'w_codes')
     w_scale = _vector(w_scale, n, dev, 'w_scale')
     if bias is not None:
         bias = _vector(bias, n, dev, 'bias')
