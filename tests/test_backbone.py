@@ -230,3 +230,17 @@ def test_conv_blocks_match_the_numpy_restatement_cpu():
 def test_conv_blocks_match_the_numpy_restatement_on_miopen(gpu):
     """The same on the MI355X (MIOpen convolutions, channels_last): 1e-4, fp32 against float64."""
     _conv_blocks_match(gpu, 1e-4)
+
+
+def test_a_block_takes_units_of_any_kind():
+    class Twice(torch.nn.Module):
+        def forward(self, x):
+            return 2 * x
+    torch.manual_seed(1)
+    block = bb.DarknetBlock(4, 8, 3)
+    block.units[0], block.units[1] = Twice(), torch.nn.Sequential(torch.nn.Identity())
+    block.units[2] = torch.nn.Sequential(torch.nn.Identity(), torch.nn.ReLU())
+    x = torch.randn(2, 4, 6, 6)
+    want = 6 * block.down(x)
+    want = want + want.relu()
+    assert torch.allclose(block(x), want, rtol=1e-6, atol=1e-6)

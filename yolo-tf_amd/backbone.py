@@ -126,10 +126,16 @@ class DarknetBlock(nn.Module):
         self.units = nn.ModuleList(nn.Sequential(ConvBN(filters, filters // 2, 1), ConvBN(filters // 2, filters, 3))
                                    for _ in range(blocks))
 
+    @staticmethod
+    def _shortcut_inside(unit):
+        """Whether a unit is two layers as made above, the second with 8-bit checkpoints; any other module is called."""
+        return (type(unit) is nn.Sequential and len(unit) == 2 and type(unit[1]) is ConvBN
+                and unit[1].checkpoints == 'int8')
+
     def forward(self, x):
         x = self.down(x)
         for unit in self.units:
-            if unit[1].checkpoints == 'int8':
+            if self._shortcut_inside(unit):
                 x = unit[1](unit[0](x), residual=x)          # the shortcut inside the normalisation's kernel
             else:
                 x = x + unit(x)
