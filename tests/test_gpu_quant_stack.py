@@ -277,3 +277,74 @@ def test_options_are_checked():
         bb.Darknet19Head(2, 1, pointwise='int4')
     with pytest.raises(ValueError, match='checkpoints'):
         bb.Darknet53Heads(2, 3, checkpoints='bf16')
+
+
+OPTIONS = [('float32', 'int8'), ('int8', 'float32'), ('int8', 'int8')]
+
+
+@pytest.mark.parametrize('pointwise,checkpoints', OPTIONS)
+def test_a_layer_whose_weights_a_hook_makes(gpu, pointwise, checkpoints):
+    """torch.nn.utils.prune sets conv.weight in a hook before each call."""
+    from torch.nn.utils import prune
+    torch.manual_seed(34)
+    layers = [_layer(32, 24, 1, 1, True, *mode, gpu) for mode in (('float32', 'float32'), (pointwise, checkpoints))]
+    layers[1].load_state_dict(layers[0].state_dict())
+    x = torch.randn(2, 32, 9, 7, device=gpu)
+    fresh, mask = torch.randn(24, 32, 1, 1, device=gpu), torch.rand(24, 32, 1, 1, device=gpu) > 0.5
+    for layer in layers:
+        prune.custom_from_mask(layer.conv, 'weight', mask)
+        with torch.no_grad():
+            layer.conv.weight_orig.copy_(fresh)
+    want, got = (layer(x) for layer in layers)
+    # as the stack's golden values are compared: the same convolution, the normalisation in float32
+    assert torch.allclose(got, want, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize('pointwise,checkpoints', OPTIONS)
+def test_hooks_of_the_modules_inside_run(gpu, pointwise, checkpoints):
+    torch.manual_seed(35)
+    block = bb.DarknetBlock(16, 32, 1)
+    for m in block.modules():
+        if isinstance(m, bb.ConvBN):
+            m.pointwise, m.checkpoints = pointwise, checkpoints
+    block.to(gpu).train()
+    x, seen = torch.randn(2, 16, 8, 8, device=gpu), []
+    want = block(x)
+    unit = block.units[0]
+    for name, m in (('unit', unit), ('second', unit[1]), ('conv', unit[0].conv), ('bn', unit[0].bn)):
+        m.register_forward_hook(lambda m, a, out, name=name: seen.append((name, out)))
+    got = block(x)
+    seen = dict(seen)
+    assert set(seen) == {'unit', 'second', 'conv', 'bn'}
+    down = block.down(x)
+    assert torch.equal(seen['unit'], seen['second']) and torch.allclose(down + seen['unit'], got, rtol=1e-5, atol=1e-5)
+    if pointwise == 'float32':
+        assert torch.allclose(got, want, rtol=1e-4, atol=1e-4)
+
+
+class _HalvedConv(torch.nn.Conv2d):
+    def forward(self, x):
+        return super().forward(x) * torch.linspace(0, 1, x.shape[-1], device=x.device)
+
+
+class _ShiftedNorm(torch.nn.BatchNorm2d):
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+@pytest.mark.parametrize('pointwise,checkpoints', OPTIONS)
+@pytest.mark.parametrize('swap', ['conv', 'dilation', 'bn'])
+def test_modules_put_in_the_place_of_a_layers_own_are_called(gpu, swap, pointwise, checkpoints):
+    torch.manual_seed(36)
+    layers = [_layer(32, 24, 1 if swap != 'dilation' else 3, 1, True, *mode, gpu) for mode in (('float32', 'float32'), (pointwise, checkpoints))]
+    x = torch.randn(2, 32, 9, 7, device=gpu)
+    new = {'conv': lambda: _HalvedConv(32, 24, 1), 'dilation': lambda: torch.nn.Conv2d(32, 24, 3, dilation=2),
+           'bn': lambda: _ShiftedNorm(24)}[swap]
+    for layer in layers:
+        setattr(layer, 'conv' if swap in ('conv', 'dilation') else 'bn', new().to(gpu))
+    layers[1].load_state_dict(layers[0].state_dict())
+    want, got = (layer(x) for layer in layers)
+    if swap in ('conv', 'dilation') or pointwise == 'float32':
+        assert torch.allclose(got, want, rtol=1e-4, atol=1e-4)
+    else:                        # the codes of both operands: 0.7 % each of a deviation, five times that at the most of 24 x 126
+        assert float((got - want).abs().max()) < 0.1

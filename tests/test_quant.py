@@ -204,3 +204,25 @@ def test_channel_counts_that_do_not_fit_a_call_are_refused(monkeypatch):
                 call()
             assert refusal.value.code == _abi.YH_ERR_LIMIT
     assert quant._rows(meta(3, most), 'x')[1:] == (3, most, most)
+
+
+def test_a_convolution_with_hooks_or_of_another_kind_is_called():
+    """... by a layer that would otherwise run its product in integers, which the CPU refuses."""
+    from yolo_tf_amd import backbone as bb
+
+    class Doubled(torch.nn.Conv2d):
+        def forward(self, x):
+            return 2 * super().forward(x)
+    x, seen = torch.randn(2, 8, 5, 5, requires_grad=True), []
+    for change in (lambda m: m.conv.register_forward_hook(lambda *a: seen.append('after')),
+                   lambda m: m.conv.register_forward_pre_hook(lambda *a: seen.append('before')),
+                   lambda m: m.conv.register_full_backward_hook(lambda *a: seen.append('backward')),
+                   lambda m: setattr(m, 'conv', Doubled(8, 4, 1)), lambda m: setattr(m, 'conv', torch.nn.Conv2d(8, 4, 1, groups=4)),
+                   lambda m: setattr(m.conv, 'forward', lambda x: x[:, :4])):
+        layer = bb.ConvBN(8, 4, 1)
+        layer.pointwise = 'int8'
+        with pytest.raises(RuntimeError, match='no CPU path'):
+            layer(x)
+        change(layer)
+        layer(x).sum().backward()
+    assert sorted(seen) == ['after', 'backward', 'before']

@@ -35,6 +35,9 @@ need a HIP device, and are float32 training on MIOpen without them):
     value in seven bits).  The forward pass is computed as before, the
     normalisation by the library's own kernels.  Three float32 tensors a layer
     (12 bytes a value) become two bytes.
+The options hold for the layers as they are made here.  A convolution,
+normalisation or residual unit that is replaced by another module, or that has
+hooks, is called as it is, without them.
 """
 import math
 import os
@@ -76,6 +79,12 @@ def _variance_scaling_(weight):
     nn.init.trunc_normal_(weight, mean=0.0, std=std, a=-2.0 * std, b=2.0 * std)
 
 
+def _as_made(module, kind):
+    """Whether calling `module` does what `kind` does and no more: neither a forward of its own nor hooks."""
+    return (getattr(module.forward, '__func__', None) is kind.forward
+            and not (module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks or module._backward_hooks))
+
+
 class ConvBN(nn.Module):
     """conv2d('same', bias) -> batch normalisation -> optional leaky ReLU(0.1):
     _conv_layer of YOLOv3.py:496-509; YOLOv2.py:355-366 without the activation,
@@ -95,16 +104,23 @@ class ConvBN(nn.Module):
             nn.init.xavier_uniform_(self.conv.weight)
         nn.init.zeros_(self.conv.bias)
 
+    def _conv_as_made(self):
+        conv, k, s = self.conv, self.kernel, self.stride
+        return (_as_made(conv, nn.Conv2d) and (conv.kernel_size, conv.stride, conv.padding, conv.dilation, conv.groups)
+                == ((k, k), (s, s), (0, 0), (1, 1), 1))
+
     def forward(self, x, residual=None):
+        # A convolution or normalisation put in the place of the layer's own, or one with hooks (which may make its
+        # weights), is called as it is.
         x = _pad_same(x, self.kernel, self.stride)
-        if self.pointwise == 'int8' and self.kernel == 1 and self.stride == 1:
+        if self.pointwise == 'int8' and self.kernel == 1 and self.stride == 1 and self._conv_as_made():
             weight = self.conv.weight.reshape(self.conv.out_channels, -1)
             x = quant.linear_int8(x.permute(0, 2, 3, 1), weight, self.conv.bias).permute(0, 3, 1, 2)
-        elif self.checkpoints == 'int8':
+        elif self.checkpoints == 'int8' and self._conv_as_made():
             x = quant.conv_kept(x, self.conv.weight, self.conv.bias, self.stride)
         else:
             x = self.conv(x)
-        if self.checkpoints == 'int8' and self.bn.training:
+        if self.checkpoints == 'int8' and self.bn.training and _as_made(self.bn, nn.BatchNorm2d):
             self.bn.num_batches_tracked.add_(1)
             return quant.norm_act_kept(x.permute(0, 2, 3, 1), self.bn.weight, self.bn.bias, self.bn.eps,
                                        LEAKY_SLOPE if self.activation else 1.0,
@@ -129,7 +145,7 @@ class DarknetBlock(nn.Module):
     @staticmethod
     def _shortcut_inside(unit):
         """Whether a unit is two layers as made above, the second with 8-bit checkpoints; any other module is called."""
-        return (type(unit) is nn.Sequential and len(unit) == 2 and type(unit[1]) is ConvBN
+        return (_as_made(unit, nn.Sequential) and len(unit) == 2 and _as_made(unit[1], ConvBN)
                 and unit[1].checkpoints == 'int8')
 
     def forward(self, x):
