@@ -348,3 +348,33 @@ def test_modules_put_in_the_place_of_a_layers_own_are_called(gpu, swap, pointwis
         assert torch.allclose(got, want, rtol=1e-4, atol=1e-4)
     else:                        # the codes of both operands: 0.7 % each of a deviation, five times that at the most of 24 x 126
         assert float((got - want).abs().max()) < 0.1
+
+
+def test_cumulative_statistics(gpu):
+    """momentum None: running statistics are the batches' mean, as torch.optim.swa_utils.update_bn sets it."""
+    from torch.optim.swa_utils import update_bn
+    torch.manual_seed(37)
+    plain = _layer(16, 24, 3, 1, True, 'float32', 'float32', gpu)
+    kept = _layer(16, 24, 3, 1, True, 'float32', 'int8', gpu)
+    kept.load_state_dict(plain.state_dict())
+    batches = [torch.randn(3, 16, 10, 9, device=gpu) * (i + 1) for i in range(3)]
+    for layer in (plain, kept):
+        update_bn(batches, layer)
+    assert int(kept.bn.num_batches_tracked) == 3
+    for name in ('running_mean', 'running_var'):
+        assert torch.allclose(getattr(plain.bn, name), getattr(kept.bn, name), rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize('change', [dict(affine=False), dict(track_running_stats=False), dict(momentum=None)])
+def test_normalisations_of_other_settings(gpu, change):
+    torch.manual_seed(38)
+    layers = [_layer(16, 24, 3, 1, True, 'float32', mode, gpu) for mode in ('float32', 'int8')]
+    for layer in layers:
+        layer.bn = torch.nn.BatchNorm2d(24, **change).to(gpu)
+    layers[1].load_state_dict(layers[0].state_dict())
+    for _ in range(2):
+        x = torch.randn(2, 16, 9, 7, device=gpu)
+        want, got = (layer(x) for layer in layers)
+        assert torch.allclose(got, want, rtol=1e-4, atol=1e-4)
+    for (name, a), (_, b) in zip(layers[0].named_buffers(), layers[1].named_buffers()):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-6), name

@@ -109,6 +109,11 @@ class ConvBN(nn.Module):
         return (_as_made(conv, nn.Conv2d) and (conv.kernel_size, conv.stride, conv.padding, conv.dilation, conv.groups)
                 == ((k, k), (s, s), (0, 0), (1, 1), 1))
 
+    def _norm_as_made(self):
+        # cumulative statistics (momentum None) are torch's to count
+        bn = self.bn
+        return _as_made(bn, nn.BatchNorm2d) and bn.affine and bn.track_running_stats and bn.momentum is not None
+
     def forward(self, x, residual=None):
         # A convolution or normalisation put in the place of the layer's own, or one with hooks (which may make its
         # weights), is called as it is.
@@ -120,7 +125,7 @@ class ConvBN(nn.Module):
             x = quant.conv_kept(x, self.conv.weight, self.conv.bias, self.stride)
         else:
             x = self.conv(x)
-        if self.checkpoints == 'int8' and self.bn.training and _as_made(self.bn, nn.BatchNorm2d):
+        if self.checkpoints == 'int8' and self.bn.training and self._norm_as_made():
             self.bn.num_batches_tracked.add_(1)
             return quant.norm_act_kept(x.permute(0, 2, 3, 1), self.bn.weight, self.bn.bias, self.bn.eps,
                                        LEAKY_SLOPE if self.activation else 1.0,
