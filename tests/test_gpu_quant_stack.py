@@ -378,3 +378,21 @@ def test_normalisations_of_other_settings(gpu, change):
         assert torch.allclose(got, want, rtol=1e-4, atol=1e-4)
     for (name, a), (_, b) in zip(layers[0].named_buffers(), layers[1].named_buffers()):
         assert torch.allclose(a, b, rtol=1e-5, atol=1e-6), name
+
+
+@pytest.mark.parametrize('autocast', [False, True])
+@pytest.mark.parametrize('kind', ['type', 'broadcast'])
+def test_a_shortcut_of_another_type_or_shape_is_added_as_by_the_plain_layer(gpu, kind, autocast):
+    """The plain layer's sum promotes and broadcasts."""
+    torch.manual_seed(31)
+    layer = _layer(16, 24, 3, 1, True, 'float32', 'int8', gpu)
+    x = torch.randn(2, 16, 9, 7, device=gpu)
+    shape = (2, 24, 9, 7) if kind == 'type' else (1, 24, 1, 1)
+    res = torch.randn(shape, device=gpu, dtype=torch.float32 if autocast else torch.float64 if kind == 'type' else torch.float32).requires_grad_()
+    with torch.autocast('cuda', dtype=torch.bfloat16, enabled=autocast):
+        out, alone = layer(x, residual=res), layer(x)
+    assert out.dtype == (torch.result_type(res, alone)) and torch.equal(out, res + alone)
+    da = torch.randn_like(out)
+    out.backward(da)
+    assert torch.equal(res.grad, da.sum_to_size(shape))
+    assert all(torch.isfinite(p.grad).all() for p in layer.parameters())

@@ -127,13 +127,18 @@ class ConvBN(nn.Module):
             x = self.conv(x)
         if self.checkpoints == 'int8' and self.bn.training and self._norm_as_made():
             self.bn.num_batches_tracked.add_(1)
-            return quant.norm_act_kept(x.permute(0, 2, 3, 1), self.bn.weight, self.bn.bias, self.bn.eps,
-                                       LEAKY_SLOPE if self.activation else 1.0,
-                                       None if residual is None else residual.permute(0, 2, 3, 1),
-                                       (self.bn.running_mean, self.bn.running_var), self.bn.momentum).permute(0, 3, 1, 2)
-        x = self.bn(x)
-        if self.activation:
-            x = F.leaky_relu(x, LEAKY_SLOPE)
+            # the kernel adds a shortcut of the result's own type and shape; any other is promoted and broadcast below
+            inside = residual is not None and residual.dtype == x.dtype and residual.shape == x.shape
+            x = quant.norm_act_kept(x.permute(0, 2, 3, 1), self.bn.weight, self.bn.bias, self.bn.eps,
+                                    LEAKY_SLOPE if self.activation else 1.0,
+                                    residual.permute(0, 2, 3, 1) if inside else None,
+                                    (self.bn.running_mean, self.bn.running_var), self.bn.momentum).permute(0, 3, 1, 2)
+            if inside:
+                return x
+        else:
+            x = self.bn(x)
+            if self.activation:
+                x = F.leaky_relu(x, LEAKY_SLOPE)
         return x if residual is None else residual + x
 
 
