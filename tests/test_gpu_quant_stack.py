@@ -396,3 +396,20 @@ def test_a_shortcut_of_another_type_or_shape_is_added_as_by_the_plain_layer(gpu,
     out.backward(da)
     assert torch.equal(res.grad, da.sum_to_size(shape))
     assert all(torch.isfinite(p.grad).all() for p in layer.parameters())
+
+
+@pytest.mark.parametrize('checkpoints', ['float32', 'int8'])
+def test_a_pointwise_layer_under_autocast_takes_the_types_of_the_plain_one(gpu, checkpoints):
+    torch.manual_seed(32)
+    layer = _layer(32, 48, 1, 1, True, 'int8', checkpoints, gpu)
+    plain = _layer(32, 48, 1, 1, True, 'float32', 'float32', gpu)
+    plain.load_state_dict(layer.state_dict())
+    x = torch.randn(2, 32, 12, 12, device=gpu).requires_grad_()
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        out, want = layer(x), plain(x)
+        half = layer(x.detach().bfloat16())
+        assert layer(x.detach().half()).dtype == plain(x.detach().half()).dtype == torch.bfloat16
+    assert out.dtype == want.dtype == torch.bfloat16
+    assert torch.equal(out, half)
+    out.sum().backward()
+    assert x.grad.dtype == torch.float32 and all(p.grad.dtype == torch.float32 and torch.isfinite(p.grad).all() for p in layer.parameters())

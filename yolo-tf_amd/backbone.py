@@ -119,6 +119,8 @@ class ConvBN(nn.Module):
         # weights), is called as it is.
         x = _pad_same(x, self.kernel, self.stride)
         if self.pointwise == 'int8' and self.kernel == 1 and self.stride == 1 and self._conv_as_made():
+            if torch.is_autocast_enabled('cuda') and x.dtype != torch.float64:
+                x = x.to(torch.get_autocast_dtype('cuda'))           # as the convolution would; linear_int8 keeps x's type
             weight = self.conv.weight.reshape(self.conv.out_channels, -1)
             x = quant.linear_int8(x.permute(0, 2, 3, 1), weight, self.conv.bias).permute(0, 3, 1, 2)
         elif self.checkpoints == 'int8' and self._conv_as_made():

@@ -341,7 +341,8 @@ class _LinearInt8(Function):
 
 def linear_int8(x, weight, bias=None):
     """x [..., K] times weight [N, K] (float, quantised by its rows in the call) plus bias, in 8-bit integers, with
-    gradients: the codes of x are the checkpoint that the weights' gradient is computed from."""
+    gradients: the codes of x are the checkpoint that the weights' gradient is computed from.  The result has x's type,
+    under autocast too."""
     return _LinearInt8.apply(x, weight, bias, torch.is_grad_enabled())
 
 
