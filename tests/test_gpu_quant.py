@@ -647,3 +647,33 @@ def test_the_backward_pass_reads_gamma_as_it_is_now(gpu):
         second = quant.norm_act_backward(da, kept)
         assert torch.equal(second[0], 2 * first[0])
         assert torch.equal(second[1], first[1]) and torch.equal(second[2], first[2])
+
+
+def test_four_threads_all_finish_with_the_right_values(gpu):
+    """Each of four threads on a stream of its own makes its 50 calls; an error in one of them is an error here."""
+    from concurrent.futures import ThreadPoolExecutor
+    rng = np.random.default_rng(38)
+    layer = lambda k, n: quant.quantize_rows(torch.from_numpy(rng.standard_normal((n, k)).astype(np.float32)).to(gpu))
+    x = [torch.randn(5000, 256, device=gpu), torch.randn(300, 512, device=gpu)]
+    dy = [torch.randn(5000, 96, device=gpu), torch.randn(300, 70, device=gpu)]
+    w = [layer(256, 96), layer(512, 70)]
+    g, b = torch.rand(256, device=gpu), torch.rand(256, device=gpu)
+
+    def calls(i):
+        y, codes, scale = quant.matmul_int8(x[i], *w[i], want_codes=True)
+        out = [y, quant.weight_grad(dy[i], codes, scale), quant.input_grad(dy[i], *w[i])]
+        if i == 0:
+            a, kept = quant.norm_act(x[0], g, b, 1e-3, 0.1)
+            out += [a, *quant.norm_act_backward(a, kept)]
+        return out
+    want = [calls(0), calls(1)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        done = 0
+        with torch.cuda.stream(torch.cuda.Stream(gpu)):
+            for _ in range(50):
+                done += all(torch.equal(a, c) for a, c in zip(calls(i % 2), want[i % 2]))
+        return done
+    with ThreadPoolExecutor(4) as pool:
+        assert [f.result() for f in [pool.submit(work, i) for i in range(4)]] == [50] * 4

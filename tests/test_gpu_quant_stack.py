@@ -413,3 +413,32 @@ def test_a_pointwise_layer_under_autocast_takes_the_types_of_the_plain_one(gpu, 
     assert torch.equal(out, half)
     out.sum().backward()
     assert x.grad.dtype == torch.float32 and all(p.grad.dtype == torch.float32 and torch.isfinite(p.grad).all() for p in layer.parameters())
+
+
+@pytest.mark.parametrize('pointwise,checkpoints', OPTIONS)
+def test_a_residual_block_under_autocast(gpu, pointwise, checkpoints):
+    """Forward and backward of a block with shortcuts: types, and the distance to the plain block under the same autocast.
+    A rounding of relative size e (codes: a row's largest is about three deviations, so 3 / 127 / sqrt(12) = 0.7 % for each
+    operand of a product; bfloat16 0.2 %) moves that share of the activations' inputs across zero, e * 0.8 of them, and each
+    takes 0.9 of its gradient along: sqrt(0.008 * 0.8) * 0.9 = 7 % in the gradient for each of five layers on either path,
+    16 % if they are independent; three times that for their correlation."""
+    grads = {}
+    x = torch.randn(2, 16, 16, 16, device=gpu)
+    da = torch.randn(2, 32, 8, 8, device=gpu)
+    for mode in (('float32', 'float32'), (pointwise, checkpoints)):
+        torch.manual_seed(33)
+        block = bb.DarknetBlock(16, 32, 2)
+        for m in block.modules():
+            if isinstance(m, bb.ConvBN):
+                m.pointwise, m.checkpoints = mode
+        block.to(gpu).to(memory_format=torch.channels_last).train()
+        with torch.autocast('cuda', dtype=torch.bfloat16):
+            out = block(x)
+        assert out.dtype == torch.bfloat16
+        (out.float() * da).sum().backward()
+        grads[mode] = {n: p.grad for n, p in block.named_parameters()}
+    for name, want in grads['float32', 'float32'].items():
+        got = grads[pointwise, checkpoints][name]
+        assert got.dtype == torch.float32 and torch.isfinite(got).all()
+        if not name.endswith('conv.bias'):                       # zero but for roundings: the normalisation takes the mean off
+            assert float((got - want).norm() / want.norm()) < 0.5, name
