@@ -1000,14 +1000,6 @@ __global__ __launch_bounds__(kThreads * kTeams, kTeams > 1 ? 1 : 3) void k_input
                                                                    0, n, dx, lddx, nullptr, nullptr);
 }
 
-template <class F>
-void with_type(int32_t type, F f)
-{
-    if (type == YH_FLOAT32) f(float());
-    else if (type == YH_BFLOAT16) f((__bf16)0.0f);
-    else f((_Float16)0.0f);
-}
-
 // Tiles of 64 x 16 tb values.  The widest reads and splits the float operand least often, which pays where each of 512
 // workgroups has 16 steps of 32 rows and more and the tiles are filled (1024 x 512 weights from 10816 rows: 48 us in all
 // with tb = 16, 53 with 8; from 2704 rows 512 x 256: 17.7 and 16.3; 384 x 255 from 43264 rows: 43.9 and 41.6).
@@ -1029,17 +1021,6 @@ GradPlan plan_weight_grad(int64_t rows, int n, int k)
 }
 
 unsigned blocks_for(int64_t count) { return (unsigned)((count + kThreads - 1) / kThreads); }
-
-}  // namespace
-
-namespace {
-
-int pow2_at_least(int v)
-{
-    int p = 1;
-    while (p < v) p <<= 1;
-    return p;
-}
 
 // How a product is computed.  All three give the same bits: the sums are whole numbers.
 struct ProductPlan {
@@ -1193,9 +1174,8 @@ hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, 
 }
 
 hipError_t launch_input_grad(const Rows &dy, const int8_t *w, int64_t ldw, const float *w_scale, int64_t rows,
-                             int32_t n, int32_t k, void *dx, int64_t lddx, int32_t type, hipStream_t st)
+                             int32_t n, int32_t k, void *dx, int64_t lddx, hipStream_t st)
 {
-    (void)type;
     with_type(dy.type, [&](auto t) {
         using T = decltype(t);
 #define CALL(TB, TEAMS)                                                                                                     \

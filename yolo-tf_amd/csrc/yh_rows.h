@@ -42,7 +42,24 @@ size_t weight_grad_workspace(int64_t rows, int32_t n, int32_t k);     // bytes
 hipError_t launch_weight_grad(const Rows &dy, const int8_t *codes, int64_t ldc, const float *scale, int64_t rows,
                               int32_t n, int32_t k, float *dw, float *db, void *workspace, hipStream_t st);
 hipError_t launch_input_grad(const Rows &dy, const int8_t *w, int64_t ldw, const float *w_scale, int64_t rows,
-                             int32_t n, int32_t k, void *dx, int64_t lddx, int32_t type, hipStream_t st);
+                             int32_t n, int32_t k, void *dx, int64_t lddx, hipStream_t st);
+
+// ---- for the launchers ---------------------------------------------------
+inline int pow2_at_least(int v)
+{
+    int p = 1;
+    while (p < v) p <<= 1;
+    return p;
+}
+
+// Calls f(T()) with the C++ type of a yh_dtype.
+template <class F>
+void with_type(int32_t type, F f)
+{
+    if (type == YH_FLOAT32) f(float());
+    else if (type == YH_BFLOAT16) f((__bf16)0.0f);
+    else f((_Float16)0.0f);
+}
 
 // ---- device helpers ------------------------------------------------------
 constexpr float kRowMin = 0x1p-110f;      // a row whose largest value is below this is zero: its scale stays a normal number

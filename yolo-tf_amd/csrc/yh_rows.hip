@@ -8,13 +8,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-int pow2_at_least(int v)
-{
-    int p = 1;
-    while (p < v) p <<= 1;
-    return p;
-}
-
 // How a wavefront holds rows in registers: `lanes` neighbouring lanes a row, each with `vecs` vectors of V elements,
 // `lanes` vectors apart.  `most` vectors a lane (four: 4 KiB of loads in flight a wavefront); rows shorter than that share
 // the wavefront, with at least eight lanes (128 contiguous bytes) each.  Below 2^20 lanes in all (64 wavefronts a compute
@@ -256,9 +249,7 @@ struct NormGrads {
     }
 };
 
-// Statistics: one read of z.  346112 x 128 in float32 (177 MB): 45 us (3.9 TB/s), the adding of the partials 5 us; sums
-// in float32, loads one round ahead, half or twice the workgroups: 44 to 49 us.
-// The same, and a workgroup's own channels, from `first` on, in LDS.
+// NormGrads, and a workgroup's own channels, from `first` on, in LDS.
 struct NormGradsHere {
     NormGrads out;
     float *b_here, *g_here;
@@ -271,6 +262,8 @@ struct NormGradsHere {
     }
 };
 
+// Statistics: one read of z.  346112 x 128 in float32 (177 MB): 45 us (3.9 TB/s), the adding of the partials 5 us; sums
+// in float32, loads one round ahead, half or twice the workgroups: 44 to 49 us.
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int64_t spare, int TX, double *part,
                                                          NormStats<T> out)
@@ -719,15 +712,6 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(const T *da, int64
             store_vec<T, V>(dz + row * ldz + c, v[i], cols - c);
         }
     }
-}
-
-// Calls f(T()) with the C++ type of a yh_dtype.
-template <class F>
-void with_type(int32_t type, F f)
-{
-    if (type == YH_FLOAT32) f(float());
-    else if (type == YH_BFLOAT16) f((__bf16)0.0f);
-    else f((_Float16)0.0f);
 }
 
 // The kernels' vector counts.

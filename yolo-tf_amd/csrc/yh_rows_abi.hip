@@ -173,7 +173,7 @@ int yh_input_grad(const void *dy, int32_t dtype, int64_t lddy, const int8_t *w, 
     YH_TRY(check_rows(dx, lddx, k, rows, element_size(dtype), true, "dx"));
     if (rows == 0) return YH_OK;
     YH_TRY(yh::require_device());
-    return launched(yh::launch_input_grad({dy, lddy, dtype}, w, ldw, w_scale, rows, n, k, dx, lddx, dtype, static_cast<hipStream_t>(stream)),
+    return launched(yh::launch_input_grad({dy, lddy, dtype}, w, ldw, w_scale, rows, n, k, dx, lddx, static_cast<hipStream_t>(stream)),
                     "input gradient launch");
 }
 
