@@ -442,3 +442,21 @@ def test_a_residual_block_under_autocast(gpu, pointwise, checkpoints):
         assert got.dtype == torch.float32 and torch.isfinite(got).all()
         if not name.endswith('conv.bias'):                       # zero but for roundings: the normalisation takes the mean off
             assert float((got - want).norm() / want.norm()) < 0.5, name
+
+
+@pytest.mark.parametrize('stride', [2, (2, 2), [2, 2], (1, 2), (1,)])
+def test_conv_kept_takes_the_strides_of_a_convolution(gpu, stride):
+    """The output is the plain convolution's; the gradients are those of the values that the codes stand for."""
+    torch.manual_seed(39)
+    x = torch.randn(2, 16, 11, 9, device=gpu).contiguous(memory_format=torch.channels_last).requires_grad_()
+    w, b = torch.randn(12, 16, 3, 3, device=gpu, requires_grad=True), torch.randn(12, device=gpu, requires_grad=True)
+    out = quant.conv_kept(x, w, b, stride)
+    held = quant.dequantize_rows(*quant.quantize_rows(x.permute(0, 2, 3, 1))).permute(0, 3, 1, 2).detach().requires_grad_()
+    assert torch.equal(out, F.conv2d(x, w, b, stride))
+    dy = torch.randn_like(out)
+    got = torch.autograd.grad(out, (x, w, b), dy)
+    want = torch.autograd.grad(F.conv2d(held, w, b, stride), (held, w, b), dy)
+    for g, v in zip(got, want):                              # the library's convolutions in float32 on both sides
+        assert torch.allclose(g, v, rtol=1e-4, atol=1e-3)
+    with torch.no_grad():
+        assert torch.equal(quant.conv_kept(x, w, b, stride), out)

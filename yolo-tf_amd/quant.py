@@ -366,7 +366,7 @@ class _ConvKept(Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         own = weight.to(dy.dtype)                           # under autocast the convolution ran in dy's type
         dx = dw = db = None
-        if weight.shape[2:] == (1, 1) and ctx.stride == 1:
+        if weight.shape[2:] == (1, 1) and ctx.stride == (1, 1):
             rows = dy.permute(0, 2, 3, 1)
             if need_x:
                 dx = (rows.reshape(-1, n) @ own.reshape(n, k)).view(codes.shape).permute(0, 3, 1, 2)
@@ -375,9 +375,8 @@ class _ConvKept(Function):
                 dw = dw.view(weight.shape)
         else:
             x = dequantize_rows(codes, scale, dy.dtype).permute(0, 3, 1, 2)
-            s = [ctx.stride, ctx.stride]
             dx, dw, db = torch.ops.aten.convolution_backward(dy.contiguous(memory_format=torch.channels_last), x, own, [n] if ctx.has_bias else None,
-                                                             s, [0, 0], [1, 1], False, [0, 0], 1, [need_x, need_w, need_b and ctx.has_bias])
+                                                             ctx.stride, [0, 0], [1, 1], False, [0, 0], 1, [need_x, need_w, need_b and ctx.has_bias])
         return (dx.to(ctx.dtype) if need_x else None, dw.to(weight.dtype) if need_w else None,
                 db.to(weight.dtype) if need_b and ctx.has_bias else None, None)
 
@@ -385,10 +384,11 @@ class _ConvKept(Function):
 def conv_kept(x, weight, bias, stride):
     """F.conv2d(x, weight, bias, stride) of an NCHW tensor that keeps x for the backward pass as row codes (a byte a
     value and a scale a pixel) in the place of x itself.  The output is the plain convolution's; the weights'
-    gradient is that of the values the codes stand for."""
+    gradient is that of the values the codes stand for.  stride: one number or two."""
+    stride = (int(stride),) * 2 if not isinstance(stride, (tuple, list)) else (int(stride[0]), int(stride[-1]))
     if not torch.is_grad_enabled() or x.shape[1] < KEEP_CODES_FROM:
         return F.conv2d(x, weight, bias, stride)
-    return _ConvKept.apply(x, weight, bias, int(stride))
+    return _ConvKept.apply(x, weight, bias, stride)
 
 
 class _NormAct(Function):
