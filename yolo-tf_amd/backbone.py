@@ -81,8 +81,9 @@ def _variance_scaling_(weight):
 
 def _as_made(module, kind):
     """Whether calling `module` does what `kind` does and no more: neither a forward of its own nor hooks."""
-    return (getattr(module.forward, '__func__', None) is kind.forward
-            and not (module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks or module._backward_hooks))
+    own = module.__dict__                  # a layer is asked twice a call, and small images wait for the host
+    return (type(module).forward is kind.forward and 'forward' not in own
+            and not (own['_forward_pre_hooks'] or own['_forward_hooks'] or own['_backward_pre_hooks'] or own['_backward_hooks']))
 
 
 class ConvBN(nn.Module):
@@ -104,41 +105,39 @@ class ConvBN(nn.Module):
             nn.init.xavier_uniform_(self.conv.weight)
         nn.init.zeros_(self.conv.bias)
 
-    def _conv_as_made(self):
-        conv, k, s = self.conv, self.kernel, self.stride
-        return (_as_made(conv, nn.Conv2d) and (conv.kernel_size, conv.stride, conv.padding, conv.dilation, conv.groups)
-                == ((k, k), (s, s), (0, 0), (1, 1), 1))
+    def _conv_as_made(self, conv):
+        return (_as_made(conv, nn.Conv2d) and conv.groups == 1 and conv.padding == (0, 0) and conv.dilation == (1, 1)
+                and conv.kernel_size == (self.kernel, self.kernel) and conv.stride == (self.stride, self.stride))
 
-    def _norm_as_made(self):
+    @staticmethod
+    def _norm_as_made(bn):
         # cumulative statistics (momentum None) are torch's to count
-        bn = self.bn
         return _as_made(bn, nn.BatchNorm2d) and bn.affine and bn.track_running_stats and bn.momentum is not None
 
     def forward(self, x, residual=None):
         # A convolution or normalisation put in the place of the layer's own, or one with hooks (which may make its
         # weights), is called as it is.
         x = _pad_same(x, self.kernel, self.stride)
-        if self.pointwise == 'int8' and self.kernel == 1 and self.stride == 1 and self._conv_as_made():
+        conv, bn = self.conv, self.bn
+        if self.pointwise == 'int8' and self.kernel == 1 and self.stride == 1 and self._conv_as_made(conv):
             if torch.is_autocast_enabled('cuda') and x.dtype != torch.float64:
                 x = x.to(torch.get_autocast_dtype('cuda'))           # as the convolution would; linear_int8 keeps x's type
-            weight = self.conv.weight.reshape(self.conv.out_channels, -1)
-            x = quant.linear_int8(x.permute(0, 2, 3, 1), weight, self.conv.bias).permute(0, 3, 1, 2)
-        elif self.checkpoints == 'int8' and self._conv_as_made():
-            x = quant.conv_kept(x, self.conv.weight, self.conv.bias, self.stride)
+            x = quant.linear_int8(x.permute(0, 2, 3, 1), conv.weight.reshape(conv.out_channels, -1), conv.bias).permute(0, 3, 1, 2)
+        elif self.checkpoints == 'int8' and self._conv_as_made(conv):
+            x = quant.conv_kept(x, conv.weight, conv.bias, self.stride)
         else:
-            x = self.conv(x)
-        if self.checkpoints == 'int8' and self.bn.training and self._norm_as_made():
-            self.bn.num_batches_tracked.add_(1)
+            x = conv(x)
+        if self.checkpoints == 'int8' and bn.training and self._norm_as_made(bn):
+            bn.num_batches_tracked.add_(1)
             # the kernel adds a shortcut of the result's own type and shape; any other is promoted and broadcast below
             inside = residual is not None and residual.dtype == x.dtype and residual.shape == x.shape
-            x = quant.norm_act_kept(x.permute(0, 2, 3, 1), self.bn.weight, self.bn.bias, self.bn.eps,
-                                    LEAKY_SLOPE if self.activation else 1.0,
-                                    residual.permute(0, 2, 3, 1) if inside else None,
-                                    (self.bn.running_mean, self.bn.running_var), self.bn.momentum).permute(0, 3, 1, 2)
+            x = quant.norm_act_kept(x.permute(0, 2, 3, 1), bn.weight, bn.bias, bn.eps, LEAKY_SLOPE if self.activation else 1.0,
+                                    residual.permute(0, 2, 3, 1) if inside else None, (bn.running_mean, bn.running_var),
+                                    bn.momentum).permute(0, 3, 1, 2)
             if inside:
                 return x
         else:
-            x = self.bn(x)
+            x = bn(x)
             if self.activation:
                 x = F.leaky_relu(x, LEAKY_SLOPE)
         return x if residual is None else residual + x
@@ -157,8 +156,10 @@ class DarknetBlock(nn.Module):
     @staticmethod
     def _shortcut_inside(unit):
         """Whether a unit is two layers as made above, the second with 8-bit checkpoints; any other module is called."""
-        return (_as_made(unit, nn.Sequential) and len(unit) == 2 and _as_made(unit[1], ConvBN)
-                and unit[1].checkpoints == 'int8')
+        if type(unit) is not nn.Sequential or len(unit) != 2:
+            return False
+        second = unit[1]
+        return getattr(second, 'checkpoints', None) == 'int8' and _as_made(unit, nn.Sequential) and _as_made(second, ConvBN)
 
     def forward(self, x):
         x = self.down(x)
