@@ -137,7 +137,7 @@ __device__ __forceinline__ void out_16x64(const v4i (&acc)[4], float s, const fl
 
 // The tile form, from codes in memory: 43264 rows, 1536 -> 425 56 us (1.0 POP/s, half of what a large library product
 // reaches), 21632 rows, 1024 -> 512 22.6 us.  A wavefront's 64 x 64 results ask LDS for as many cycles as the matrix
-// instructions take (counted over a launch: matrix instructions busy 25 % of the cycles, LDS 32 %).  Operands read a step
+// instructions take (counted over a launch: matrix instructions busy 24 % of the time, LDS 31 %).  Operands read a step
 // ahead win 3 to 9 % where few wavefronts share a compute unit (2704 rows, 1024 -> 512 7.6 us, 8.3 without); larger tiles,
 // longer steps, loads further ahead and wave priorities won nothing.  Three workgroups a compute unit: 168 registers.
 template <class T, int BM, int BN>
@@ -519,7 +519,7 @@ __device__ __forceinline__ void code_rows_given(const int8_t *x, int64_t ldx, co
 // Few rows: a workgroup takes 16 rows and 64 channels, 16 a wavefront.  The weights' loads are under way before the rows
 // are turned into codes (four rows a wavefront); nothing is read in turns, so a call lasts about three memory latencies
 // and one pass through its code, which is why rows of up to 256 channels have a form of their own (S = 1; 300 rows,
-// 256 -> 128: 5.0 us, 6.0 with S = 4).  169 rows, 1024 -> 512: 6.6 us.
+// 256 -> 128: 5.0 us, 6.0 with S = 4).  169 rows, 1024 -> 512: 7.0 us.
 template <class TX, class T, int S, bool kWhole>             // kWhole: K is a multiple of 16
 __global__ __launch_bounds__(kThreads) void k_int8_few(const TX *x, int64_t ldx, int64_t spare, const float *xs, int64_t rows, int k,
                                                        const int8_t *w, int64_t ldw, int64_t spare_w, const float *ws, int n, const float *bias,
@@ -941,8 +941,9 @@ __device__ __forceinline__ void split_tile(const T *dy, int64_t ldd, const float
 }
 
 // Weight gradient: workgroup (tile of dw, piece of the rows).  The pieces' results are added by k_add_pieces in a fixed
-// order (no atomics: the same bits on every run).  1024 x 512 weights from 10816 rows: 40 us (34 GFLOP as three bfloat16
-// products, 0.86 PFLOP/s) and 6.7 us for the pieces; 128 x 64 from 692224 rows: 56 us (269 MB, 4.8 TB/s) and 8 us.
+// order (no atomics: the same bits on every run).  1024 x 512 weights from 10816 rows: 41 us (34 GFLOP as three bfloat16
+// products, 0.82 PFLOP/s) and 7.3 us for the pieces; 128 x 64 from 692224 rows: 57 us (269 MB, 4.7 TB/s) and 7.4 us, from
+// bfloat16 rows 63 us (180 MB: not bound by memory).
 template <class T, int TB>
 __global__ __launch_bounds__(kThreads, 2) void k_weight_grad(const T *dy, int64_t ldd, const int8_t *codes, int64_t ldc, const float *scale,
                                                              int64_t spare, int64_t rows, int n, int k, int64_t rows_per_piece, int tiles_k, int tiles,
@@ -989,8 +990,9 @@ __global__ __launch_bounds__(kThreads) void k_fill_zero(float *p, int64_t count)
 }
 
 // Input gradient: workgroup (64 rows, 16 TB columns), the whole sum over the output channels.  Bound by the matrix
-// instructions and the vector instructions beside them: 43264 rows, 256 -> 512 in float32 42 us (34 GFLOP as three bfloat16
-// products: 0.81 PFLOP/s; the memory's share is 26 us), 21632 rows, 255 -> 128 12.5 us (2.7 TB/s).
+// instructions and the vector instructions beside them: 43264 rows, 256 -> 512 in float32 43 us (34 GFLOP as three bfloat16
+// products: 0.79 PFLOP/s; the memory's share is 26 us; 48 us a call back to back), 21632 rows, 255 -> 128 13.3 us
+// (2.5 TB/s); in bfloat16 39.5 and 11.9 us.
 template <class T, int TB, int kTeams>
 __global__ __launch_bounds__(kThreads * kTeams, kTeams > 1 ? 1 : 3) void k_input_grad(const T *dy, int64_t ldd, const int8_t *w, int64_t ldw, const float *ws,
                                                             int64_t spare, int64_t rows, int n, int k, int tiles_k, T *dx, int64_t lddx)
@@ -1184,7 +1186,7 @@ hipError_t launch_input_grad(const Rows &dy, const int8_t *w, int64_t ldw, const
             k_input_grad<T, TB, TEAMS><<<dim3((unsigned)((rows + 63) / 64 * tk)), kThreads * TEAMS, 0, st>>>(               \
                 static_cast<const T *>(dy.p), dy.ld, w, ldw, w_scale, spare_rows(n, ldw, 4), rows, n, k, tk, static_cast<T *>(dx), lddx);          \
         } while (0)
-        // Tiles of 64 x 128 (43264 rows, 256 -> 512: 40 us, 45 with 64 x 256, 51 with 64 x 64); half as wide where that gives
+        // Tiles of 64 x 128 (43264 rows, 256 -> 512: 64 x 256 takes 1.12 times as long, 64 x 64 1.27 times); half as wide where that gives
         // too few workgroups, and with the sum over four teams where even so they are few and the sum is long (169 rows,
         // 512 -> 1024, 48 workgroups: 8.2 us, 11.4 with one team; 32000 rows, 255 -> 60, 500 workgroups: 17.0 and 12.4; 2704
         // rows, 128 -> 256, four steps: 5.6 and 5.3).

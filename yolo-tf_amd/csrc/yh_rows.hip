@@ -26,7 +26,7 @@ RowPlan plan_row(int64_t rows, int cols, int V, int most)
 
 // Row codes, written: one read of x, one write of the codes; the row waits in registers for its maximum (lanes of a row
 // exchange it by data-parallel moves).  Bound by memory: 173056 x 128 in float32 20 us (112 MB, 5.6 TB/s), 43264 x 1536 in
-// bfloat16 36.5 us (5.5 TB/s).
+// bfloat16 37.6 us (5.3 TB/s; 43 where the launch before still writes).
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_quantize(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *codes, int64_t ldc,
                                                        float *scale, int lanes, int64_t spare)
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void k_quantize_long(const T *x, int64_t 
     }
 }
 
-// Row codes, read: 173056 x 128 to float32 18.8 us (111 MB, 5.9 TB/s).
+// Row codes, read: 173056 x 128 to float32 18.6 us (111 MB, 6.0 TB/s), 43264 x 1536 to bfloat16 30.2 us (200 MB, 6.6 TB/s).
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_dequantize(const int8_t *codes, int64_t ldc, const float *scale, int64_t rows, int cols,
                                                          T *out, int64_t ldo, int lanes, int64_t spare)
@@ -262,7 +262,7 @@ struct NormGradsHere {
     }
 };
 
-// Statistics: one read of z.  346112 x 128 in float32 (177 MB): 45 us (3.9 TB/s), the adding of the partials 5 us; sums
+// Statistics: one read of z.  346112 x 128 in float32 (177 MB): 46 us (3.9 TB/s), the adding of the partials 5 us; sums
 // in float32, loads one round ahead, half or twice the workgroups: 44 to 49 us.
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(const T *z, int64_t rows, int cols, int64_t ldz, int64_t spare, int TX, double *part,
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats_finish(const double *pa
 }
 
 // The elementwise pass: z (and the shortcut) in, the activation and the checkpoint out, a row's maximum between its lanes.
-// Bound by memory: 346112 x 128 in float32 with a shortcut 97 us (577 MB, 5.9 TB/s).
+// Bound by memory: 346112 x 128 in float32 with a shortcut 98 us (577 MB, 5.9 TB/s).
 template <class T, int IT>
 __global__ __launch_bounds__(kThreads) void k_norm_apply(const T *z, int64_t ldz, const T *res, int64_t ldr, int64_t rows, int cols,
                                                          const float *mean, const float *invstd, const float *gamma, const float *beta, float slope,
@@ -551,7 +551,7 @@ __device__ __forceinline__ void input_grads(float (&v)[V], const uint32_t (&w)[V
     }
 }
 
-// Sums of the backward pass: da and the checkpoint in.  346112 x 128 in float32 (223 MB): 55 us (4.0 TB/s).
+// Sums of the backward pass: da and the checkpoint in.  346112 x 128 in float32 (223 MB): 57 us (3.9 TB/s).
 template <class T>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
                                                              int64_t rows, int cols, float slope, int64_t spare, int TX, double *part,
@@ -606,8 +606,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(const T *da, int64_
 }
 
 // The whole backward pass for few rows: a workgroup holds its channels' rows, U a thread, and gives both the sums and the
-// input gradients.  169 x 1024 in bfloat16: 6.3 us, 9.3 in two
-// launches; 512 x 1024: 8.6 and 10.1.
+// input gradients.  169 x 1024 in bfloat16: 6.6 us, 9.3 in two launches; 512 x 1024: 8.6 and
+// 10.1.
 template <class T, int U>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_few(const T *da, int64_t ldd, const int8_t *kept, int64_t ldk, const float *scale,
                                                             int64_t rows, int cols, float slope, int64_t spare, int TX, const float *gamma,
