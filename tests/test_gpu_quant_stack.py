@@ -383,9 +383,9 @@ def test_normalisations_of_other_settings(gpu, change):
 @pytest.mark.parametrize('autocast', [False, True])
 @pytest.mark.parametrize('kind', ['type', 'broadcast'])
 def test_a_shortcut_of_another_type_or_shape_is_added_as_by_the_plain_layer(gpu, kind, autocast):
-    """The plain layer's sum promotes and broadcasts."""
+    """The plain layer's sum promotes and broadcasts.  The product in integers, so that two calls give the same bits."""
     torch.manual_seed(31)
-    layer = _layer(16, 24, 3, 1, True, 'float32', 'int8', gpu)
+    layer = _layer(16, 24, 1, 1, True, 'int8', 'int8', gpu)
     x = torch.randn(2, 16, 9, 7, device=gpu)
     shape = (2, 24, 9, 7) if kind == 'type' else (1, 24, 1, 1)
     res = torch.randn(shape, device=gpu, dtype=torch.float32 if autocast else torch.float64 if kind == 'type' else torch.float32).requires_grad_()
@@ -452,11 +452,12 @@ def test_conv_kept_takes_the_strides_of_a_convolution(gpu, stride):
     w, b = torch.randn(12, 16, 3, 3, device=gpu, requires_grad=True), torch.randn(12, device=gpu, requires_grad=True)
     out = quant.conv_kept(x, w, b, stride)
     held = quant.dequantize_rows(*quant.quantize_rows(x.permute(0, 2, 3, 1))).permute(0, 3, 1, 2).detach().requires_grad_()
-    assert torch.equal(out, F.conv2d(x, w, b, stride))
+    # sums of 144 terms of about 0.64 in float32, in any order: (1 + 4 sqrt(144)) 2^-24 * 92
+    assert torch.allclose(out, F.conv2d(x, w, b, stride), rtol=0, atol=3e-4)
     dy = torch.randn_like(out)
     got = torch.autograd.grad(out, (x, w, b), dy)
     want = torch.autograd.grad(F.conv2d(held, w, b, stride), (held, w, b), dy)
     for g, v in zip(got, want):                              # the library's convolutions in float32 on both sides
         assert torch.allclose(g, v, rtol=1e-4, atol=1e-3)
     with torch.no_grad():
-        assert torch.equal(quant.conv_kept(x, w, b, stride), out)
+        assert torch.allclose(quant.conv_kept(x, w, b, stride), out, rtol=0, atol=3e-4)
